@@ -27,6 +27,7 @@ TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q5_0 = 0, 1, 2, 6
 TYPE_Q8_0 = 8
 TYPE_Q4_K = 12
 TYPE_Q5_K, TYPE_Q6_K = 13, 14
+TYPE_BF16 = 30  # paged caches only
 QK8_0, QK_K = 32, 256
 ORDER_X86, ORDER_RELAXED = 0, 1  # EDGEXPU_CUDA_ORDER_* (include/edgexpu_cuda.h)
 Q8_0_BYTES, Q8_K_BYTES, Q4_K_BYTES = 34, 292, 144
@@ -49,6 +50,15 @@ class HbmPlan(ctypes.Structure):
     _fields_ = [("weight_bytes", ctypes.c_uint64), ("kv_bytes", ctypes.c_uint64), ("scratch_bytes", ctypes.c_uint64),
                 ("total_bytes", ctypes.c_uint64), ("limit_bytes", ctypes.c_uint64), ("file_bytes", ctypes.c_uint64),
                 ("window", ctypes.c_int), ("admitted", ctypes.c_int), ("reason", ctypes.c_char * 256)]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """edgexpu_cuda_kv_cache (include/edgexpu_cuda.h); ``kv.KvCache`` fills it from torch tensors."""
+
+    _fields_ = [("k", _c_vp), ("v", _c_vp), ("layer_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("type", _c_u32), ("n_layers", _c_int), ("n_pages", _c_int), ("page_size", _c_int), ("n_kv", _c_int),
+                ("head_dim", _c_int), ("n_seqs", _c_int), ("max_pages", _c_int), ("table", _c_vp), ("lens", _c_vp),
+                ("refs", _c_vp), ("work", _c_vp)]
 
 
 _CUDA_SIGS = {
@@ -104,6 +114,19 @@ _CUDA_SIGS = {
     "edgexpu_cuda_llama_forward": (_c_int, [_c_vp, _c_vp, _c_int, _c_int, ctypes.c_float, ctypes.c_float, _c_u64p,
                                             ctypes.POINTER(_c_u32), _c_vp, _c_str, _c_sz]),
     "edgexpu_cuda_llama_close": (_c_int, [_c_vp]),
+    "edgexpu_cuda_kv_work_bytes": (_c_sz, [_c_int, _c_int]),
+    "edgexpu_cuda_kv_append_dev": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp]),
+    "edgexpu_cuda_kv_fork_dev": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp]),
+    "edgexpu_cuda_kv_free_dev": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp]),
+    "edgexpu_cuda_kv_copy_dev": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp]),
+    "edgexpu_cuda_kv_compact_dev": (_c_int, [_c_vp, _c_vp, _c_vp]),
+    "edgexpu_cuda_qk_norm_rope_dev": (
+        _c_int, [_c_vp, _c_int, _c_vp, _c_vp, _c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _c_int, _c_int, _c_vp,
+                 _c_vp, ctypes.c_float, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "edgexpu_cuda_kv_attention_dev": (
+        _c_int, [_c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.c_float, _c_vp,
+                 _c_u32, _c_vp, _c_sz, _c_vp]),
+    "edgexpu_cuda_kv_attention_work_bytes": (_c_sz, [_c_vp, _c_int, _c_int, _c_int, _c_int, _c_int]),
 }
 
 _HOST_SIGS = {

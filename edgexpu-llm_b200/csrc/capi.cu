@@ -564,12 +564,14 @@ int check_status(char* error, size_t error_size) {
     const uint32_t s = *g.h_status;
     *g.h_status = 0;
     cudaMemset(g.d_status, 0, sizeof(uint32_t));
-    return fail(error, error_size, "device status 0x%x:%s%s%s%s%s", s,
+    return fail(error, error_size, "device status 0x%x:%s%s%s%s%s%s%s", s,
                 (s & ex::ST_TIMEOUT_FULL) ? " a consumer gave up waiting for a tile copy;" : "",
                 (s & ex::ST_TIMEOUT_EMPTY) ? " the producer gave up waiting for a free stage;" : "",
                 (s & ex::ST_TIMEOUT_DRAIN) ? " copies were still in flight at exit;" : "",
                 (s & ex::ST_TIMEOUT_PEER) ? " a tensor-parallel peer did not deliver its partial in time;" : "",
-                (s & ex::ST_BAD_INDEX) ? " a row id was outside the tensor;" : "");
+                (s & ex::ST_BAD_INDEX) ? " a row id was outside the tensor;" : "",
+                (s & ex::ST_BAD_CACHE) ? " a sequence, position or page was outside its cache;" : "",
+                (s & ex::ST_NO_PAGES) ? " a cache had too few free pages;" : "");
   }
   return 1;
 }

@@ -35,6 +35,7 @@ constexpr uint32_t TYPE_Q8_0 = 8;
 constexpr uint32_t TYPE_Q4_K = 12;
 constexpr uint32_t TYPE_Q5_K = 13;
 constexpr uint32_t TYPE_Q6_K = 14;
+constexpr uint32_t TYPE_BF16 = 30;
 
 // Bits of the device status word (host-mapped; kernels only ever OR into it).
 constexpr uint32_t ST_TIMEOUT_FULL = 1u;   // a consumer gave up waiting for a tile copy
@@ -42,6 +43,8 @@ constexpr uint32_t ST_TIMEOUT_EMPTY = 2u;  // the producer gave up waiting for a
 constexpr uint32_t ST_TIMEOUT_DRAIN = 4u;  // copies still in flight at exit after the limit
 constexpr uint32_t ST_TIMEOUT_PEER = 8u;   // a tensor-parallel peer did not deliver its partial in time
 constexpr uint32_t ST_BAD_INDEX = 16u;     // a row id passed to a gather was outside the tensor
+constexpr uint32_t ST_BAD_CACHE = 32u;     // a sequence, position or page was outside its paged cache
+constexpr uint32_t ST_NO_PAGES = 64u;      // a paged cache had too few free pages for an append
 
 // Every mbarrier wait gives up after this long and reports through the status word.
 constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;  // 2 s

@@ -1,0 +1,675 @@
+// kvattn.cu -- attention of a batch's last tokens over a paged cache, with a prefix that all its
+// sequences share read once.
+//
+// Mathematics.  The softmax of a row over a set of positions is the join of its parts: with, for each
+// part, m = max s_j, l = sum 2^(s_j - m) and o = sum 2^(s_j - m) v_j (scores in log2 units), the whole
+// is M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L.  So the queries of all sequences that
+// share a prefix are stacked into one matrix against it (rows = tokens x heads of the group), each
+// sequence's own positions are a second part, long parts are split further, and a last kernel joins.
+//
+// A row's mask is a number, the positions it sees.  Positions outside a block's range are loaded as
+// zeros, so memory past a sequence's end may hold anything.  A sequence one of whose tokens sees less
+// than the whole prefix takes no part in the shared pass: its own pass starts at position 0, which
+// keeps the shared pass free of masks by row.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <mutex>
+
+#include "capi_internal.h"
+#include "kv.cuh"
+
+namespace ex {
+namespace {
+
+constexpr int TILE = 64;       // positions a tile, a multiple of 64 from position 0: a page never straddles two
+constexpr int MAX_SLOTS = 64;  // parts of a row in the shared pass, and in its own
+// Softmax weights are kept 2^P_SHIFT times as large, in o and l alike, so that f16 holds the small
+// weights of a long row in full: 2^-26 of the largest and more, where 2^-14 would be its limit.
+constexpr float P_SHIFT = 12.0f;
+
+struct AttnArgs {
+  KvView c;
+  long long layer_off;  // elements
+  const uint16_t* q;
+  const int32_t* seqs;
+  const int32_t* q_start;
+  int n_batch, n_tokens, n_heads, rep;
+  int shared_seq, shared_len;
+  float scale;       // times log2(e)
+  int n_pre, n_own;  // parts of the shared prefix, and of a sequence's own positions
+  float* part_o;     // [n_pre + n_own][token][head][hd]
+  float2* part_ml;   // [n_pre + n_own][token][head]: m, l
+  void* out;
+  int out_f32;
+};
+
+// Positions of the prefix.
+__device__ __forceinline__ int shared_of(const AttnArgs& a) {
+  if (a.shared_len <= 0) return 0;
+  const int held = min(a.c.lens[a.shared_seq], a.c.max_pages << a.c.ps_shift);
+  return max(0, min(a.shared_len, held));
+}
+
+struct Entry {
+  int row;         // of the table; -1: idle
+  int t0, nq;      // its tokens
+  int len;         // positions held
+  int start;       // first position of its own pass
+  bool shares;     // it takes part in the shared pass
+};
+
+__device__ __forceinline__ Entry entry_of(const AttnArgs& a, int i, int shared) {
+  Entry e{-1, i, 1, 0, 0, false};
+  if (a.q_start != nullptr) {
+    e.t0 = a.q_start[i];
+    e.nq = a.q_start[i + 1] - e.t0;
+    if (e.t0 < 0 || e.nq < 0 || e.t0 > a.n_tokens || e.nq > a.n_tokens - e.t0) {
+      atomicOr(a.c.status, ST_BAD_CACHE);
+      e.t0 = e.nq = 0;
+      return e;
+    }
+  }
+  const int s = a.seqs[i];
+  if (s < 0) return e;
+  if (s >= a.c.n_seqs) {
+    atomicOr(a.c.status, ST_BAD_CACHE);
+    return e;
+  }
+  e.row = s;
+  const int held = a.c.lens[s], most = a.c.max_pages << a.c.ps_shift;
+  if (held < 0 || held > most) atomicOr(a.c.status, ST_BAD_CACHE);
+  e.len = max(0, min(held, most));
+  e.shares = shared > 0 && e.len - e.nq + 1 >= shared;
+  e.start = e.shares ? shared : 0;
+  return e;
+}
+
+// Tiles of a part: those of [start, end) cut into at most n parts of `per` tiles.
+struct Cut {
+  int first, tiles, per, used;
+};
+__device__ __forceinline__ Cut cut_of(int start, int end, int n) {
+  Cut c;
+  c.first = start / TILE;
+  c.tiles = end > start ? (end + TILE - 1) / TILE - c.first : 0;
+  c.per = max(1, (c.tiles + n - 1) / n);
+  c.used = (c.tiles + c.per - 1) / c.per;
+  return c;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two neighbouring outputs of a row whose sums are o and weight l.  A row that sees nothing is 0; one
+// that sees only scores of -inf is 0/0, as its softmax is.
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, long long at, float o0, float o1, float l, bool sees) {
+  const float r = 1.0f / l;
+  o0 = sees ? o0 * r : 0.0f;
+  o1 = sees ? o1 * r : 0.0f;
+  if (a.out_f32)
+    *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(o0, o1);
+  else
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) = pack16<T>(o0, o1);
+}
+
+template <int DP, int WM>
+struct RowsLayout {
+  static constexpr int ROWS = 16 * WM;
+  static constexpr int STAGES = DP == 64 ? 4 : DP == 128 ? 3 : 2;
+  static constexpr int Q_BYTES = ROWS * DP * 2;
+  static constexpr int KV_BYTES = TILE * DP * 2;
+  static constexpr int JOIN_BYTES = WM == 1 ? 4 * 16 * DP * 4 : 0;  // over the stages, when they are done with
+  static constexpr int ALLOC = Q_BYTES + STAGES * 2 * KV_BYTES;
+  static_assert(JOIN_BYTES <= STAGES * 2 * KV_BYTES, "the join fits the stages");
+};
+
+// One block: 16 * WM rows of one key/value head against one part of the prefix (PRE) or of an entry's
+// own positions.  Four warps; with WM = 4 each has 16 rows and all positions of a tile, with WM = 1
+// (a single token's heads) all have the same 16 rows and 16 positions of each tile, and join at the
+// end.  Tiles come by 16-byte asynchronous copies into STAGES buffers, chunks of a row swapped by
+// row % 8 so that ldmatrix reads all banks.  P is rounded to the cache's type for its product, as the
+// tensor cores take it; its sum l is of the unrounded values.
+template <typename T, int DP, int WM>
+__global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const int pre) {
+  using L = RowsLayout<DP, WM>;
+  constexpr int ROWS = L::ROWS, NT = WM == 1 ? 2 : 8, CH = DP / 8, ST = L::STAGES;
+  pdl_enter_grid();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ unsigned long long bad_keys;
+  const uint32_t q_s = smem_u32(smem), kv_s = q_s + L::Q_BYTES;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  const int hd = a.c.hd, rep = a.rep;
+  const int shared = shared_of(a);
+
+  // the block's rows: tokens x heads of the group, from row r0 of entry e (or of the whole batch)
+  Entry e{a.shared_seq, 0, a.n_tokens, shared, 0, true};
+  int r0 = blockIdx.x * ROWS;
+  if (!pre) {
+    int i = blockIdx.x, blk = 0;
+    const int per_entry = (rep + ROWS - 1) / ROWS;
+    if (a.q_start == nullptr) {
+      i = blockIdx.x / per_entry;
+      blk = blockIdx.x - i * per_entry;
+    } else {  // the entry whose blocks hold this one: a scan of the entries' block counts, a warp wide
+      int before = 0, found = -1;
+      for (int base = 0; base < a.n_batch && found < 0; base += 32) {
+        int cnt = 0;
+        if (base + lane < a.n_batch) {
+          const Entry x = entry_of(a, base + lane, shared);
+          cnt = (x.nq * rep + ROWS - 1) / ROWS;
+        }
+        int inc = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+          if (lane >= o) inc += y;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + inc > static_cast<int>(blockIdx.x));
+        if (past != 0) {
+          const int src = __ffs(past) - 1;
+          found = base + src;
+          blk = blockIdx.x - (before + __shfl_sync(0xFFFFFFFFu, inc - cnt, src));
+        }
+        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+      }
+      if (found < 0) return;
+      i = found;
+    }
+    e = entry_of(a, i, shared);
+    r0 = blk * ROWS;
+  }
+  const int n_rows = min(ROWS, e.nq * rep - r0);
+  if (n_rows <= 0) return;
+  const bool whole = a.n_pre + a.n_own == 1;  // the only part there is: no join follows
+
+  // what the rows see: row r is token r / rep; rows past the end see what the last one does
+  const int last_tok = (r0 + n_rows - 1) / rep, first_tok = r0 / rep;
+  const int block_hi = e.row < 0 ? 0 : pre ? shared : max(0, e.len - e.nq + last_tok + 1);
+  const int block_lo_hi = e.row < 0 ? 0 : pre ? shared : max(0, e.len - e.nq + first_tok + 1);
+  const Cut cut = pre ? cut_of(0, shared, a.n_pre) : cut_of(e.start, e.row < 0 ? 0 : e.len, a.n_own);
+  if (split > 0 && split >= cut.used) return;  // the join knows
+  const int t_begin = cut.first + split * cut.per;
+  const int t_end = min(min(t_begin + cut.per, cut.first + cut.tiles), (block_hi + TILE - 1) / TILE);
+  const int wr = WM == 4 ? w * 16 : 0;  // the warp's rows of the block
+  int hi[2], tok[2], head[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = r0 + min(wr + (lane >> 2) + 8 * h, n_rows - 1);
+    tok[h] = e.t0 + r / rep;
+    head[h] = kvh * rep + r % rep;
+    hi[h] = e.row < 0 ? 0 : pre ? shared : e.len - e.nq + r / rep + 1;
+  }
+
+  const uint16_t* kb = a.c.k + a.layer_off + (static_cast<long long>(kvh) << a.c.ps_shift) * hd;
+  const uint16_t* vb = a.c.v + a.layer_off + (static_cast<long long>(kvh) << a.c.ps_shift) * hd;
+  const int32_t* table = a.c.table + static_cast<long long>(max(0, e.row)) * a.c.max_pages;
+  auto load_tile = [&](int t, int stage) {
+    const uint32_t dst = kv_s + stage * 2 * L::KV_BYTES;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < TILE * CH; i += 128) {
+      const int key = i / CH, ch = i % CH, p = t * TILE + key;
+      const bool on = p >= e.start && p < block_hi && ch * 8 < hd;
+      long long off = 0;
+      bool ok = on;
+      if (on) {
+        const int page = table[p >> a.c.ps_shift];
+        ok = page >= 0 && page < a.c.n_pages;
+        if (!ok) atomicOr(a.c.status, ST_BAD_CACHE);
+        else off = page * a.c.page_stride + static_cast<long long>(p & ((1 << a.c.ps_shift) - 1)) * hd + ch * 8;
+      }
+      const uint32_t at = dst + key * DP * 2 + ((ch ^ (key & 7)) << 4);
+      cp16(at, kb + off, ok);
+      cp16(at + L::KV_BYTES, vb + off, ok);
+    }
+  };
+
+  for (int i = threadIdx.x; i < ROWS * CH; i += 128) {
+    const int r = i / CH, ch = i % CH, rr = r0 + min(r, n_rows - 1);
+    const long long at = (static_cast<long long>(e.t0 + rr / rep) * a.n_heads + kvh * rep + rr % rep) * hd + ch * 8;
+    cp16(q_s + r * DP * 2 + ((ch ^ (r & 7)) << 4), a.q + (ch * 8 < hd ? at : 0), ch * 8 < hd);
+  }
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) {
+    if (t_begin + s < t_end) load_tile(t_begin + s, s);
+    cp_commit();
+  }
+
+  float o[DP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  const int kw = WM == 1 ? w * 16 : 0;  // the warp's positions of a tile
+  const int g = lane >> 3, lr = lane & 7;
+
+  for (int t = t_begin; t < t_end; ++t) {
+    const int stage = (t - t_begin) % ST;
+    cp_wait<ST - 2>();
+    __syncthreads();
+    if (t + ST - 1 < t_end) load_tile(t + ST - 1, (t - t_begin + ST - 1) % ST);
+    cp_commit();
+    const uint32_t ks = kv_s + stage * 2 * L::KV_BYTES, vs = ks + L::KV_BYTES;
+
+    float s[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      uint32_t qa[4];
+      const int qr = wr + lr + (g & 1) * 8, qc = 2 * kk + (g >> 1);
+      ldsm4(qa, q_s + qr * DP * 2 + ((qc ^ (qr & 7)) << 4));
+#pragma unroll
+      for (int i = 0; i < NT; i += 2) {
+        uint32_t kf[4];
+        const int key = kw + i * 8 + lr + (g >> 1) * 8, ch = 2 * kk + (g & 1);
+        ldsm4(kf, ks + key * DP * 2 + ((ch ^ (key & 7)) << 4));
+        mma16816<T>(s[i], qa, kf[0], kf[1]);
+        mma16816<T>(s[i + 1], qa, kf[2], kf[3]);
+      }
+    }
+    const int p0 = t * TILE + kw;
+    const bool masked = t * TILE < e.start || (t + 1) * TILE > block_lo_hi;
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[i][x] *= a.scale;
+        if (masked) {
+          const int p = p0 + i * 8 + (lane & 3) * 2 + (x & 1);
+          if (p < e.start || p >= hi[x >> 1]) s[i][x] = -INFINITY;
+        }
+        top[x >> 1] = fmaxf(top[x >> 1], s[i][x]);
+      }
+    float base[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 2));
+      const float mn = fmaxf(m[h], top[h]);
+      base[h] = mn == -INFINITY ? 0.0f : mn;
+      const float f = exp2f(m[h] - base[h]);
+      l[h] *= f;
+      m[h] = mn;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        o[i][2 * h] *= f;
+        o[i][2 * h + 1] *= f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[i][x] = exp2f(s[i][x] - (base[x >> 1] - P_SHIFT));
+        l[x >> 1] += s[i][x];
+      }
+    // A value that is no number, at a position that only some of the rows see: a product with a weight of
+    // 0 would spread it to the others, so it is added to the rows that see it and cleared for the product.
+    if (masked && block_lo_hi < block_hi) {
+      unsigned long long bad = 0;
+      const int from = max(0, block_lo_hi - t * TILE), n = min(TILE, block_hi - t * TILE) - from;
+      for (int x = threadIdx.x; x < n * CH; x += 128) {
+        const int key = from + x / CH, ch = x % CH;
+        const uint4 v = *reinterpret_cast<const uint4*>(smem + (vs - q_s) + key * DP * 2 + ((ch ^ (key & 7)) << 4));
+        if (!finite16<T>(v)) bad |= 1ull << key;
+      }
+      if (__syncthreads_or(bad != 0)) {
+        if (threadIdx.x == 0) bad_keys = 0;
+        __syncthreads();
+        if (bad != 0) atomicOr(&bad_keys, bad);
+        __syncthreads();
+        bad = bad_keys;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          for (int x = 0; x < 8; ++x) {
+            const int key = kw + i * 8 + x, p = t * TILE + key;
+            if (((bad >> key) & 1) == 0) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float pr = __shfl_sync(0xFFFFFFFFu, (x & 1) != 0 ? s[i][2 * h + 1] : s[i][2 * h], (lane & ~3) | (x >> 1));
+              if (p >= hi[h]) continue;
+#pragma unroll
+              for (int d = 0; d < DP / 8; ++d) {
+                const float2 v = unpack16<T>(*reinterpret_cast<const uint32_t*>(smem + (vs - q_s) + key * DP * 2 +
+                                                                                ((d ^ (key & 7)) << 4) + (lane & 3) * 4));
+                o[d][2 * h] += pr * v.x;
+                o[d][2 * h + 1] += pr * v.y;
+              }
+            }
+          }
+        __syncthreads();
+        for (int x = threadIdx.x; x < n * CH; x += 128) {
+          const int key = from + x / CH, ch = x % CH;
+          if (((bad >> key) & 1) != 0) *reinterpret_cast<uint4*>(smem + (vs - q_s) + key * DP * 2 + (ch << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncthreads();
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i += 2) {
+      const uint32_t pa[4] = {pack16<T>(s[i][0], s[i][1]), pack16<T>(s[i][2], s[i][3]), pack16<T>(s[i + 1][0], s[i + 1][1]),
+                              pack16<T>(s[i + 1][2], s[i + 1][3])};
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        uint32_t vf[4];
+        const int key = kw + i * 8 + lr + (g & 1) * 8, ch = 2 * d + (g >> 1);
+        ldsm4t(vf, vs + key * DP * 2 + ((ch ^ (key & 7)) << 4));
+        mma16816<T>(o[2 * d], pa, vf[0], vf[1]);
+        mma16816<T>(o[2 * d + 1], pa, vf[2], vf[3]);
+      }
+    }
+  }
+  cp_wait<0>();
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+  }
+
+  const int slot = (pre ? 0 : a.n_pre) + split;
+  const long long part = static_cast<long long>(slot) * a.n_tokens * a.n_heads;
+  if constexpr (WM == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (wr + (lane >> 2) + 8 * h >= n_rows) continue;
+      const long long row = static_cast<long long>(tok[h]) * a.n_heads + head[h];
+      if (!whole && (lane & 3) == 0) a.part_ml[part + row] = make_float2(m[h], l[h]);
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        const int d = i * 8 + (lane & 3) * 2;
+        if (d >= hd) continue;
+        if (whole)
+          store_out<T>(a, row * hd + d, o[i][2 * h], o[i][2 * h + 1], l[h], hi[h] > 0);
+        else
+          *reinterpret_cast<float2*>(a.part_o + (part + row) * hd + d) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+      }
+    }
+  } else {
+    // join the four warps' positions: their m and l, then their sums through shared memory
+    __shared__ float2 ml_s[4][16];
+    float* o_s = reinterpret_cast<float*>(smem + L::Q_BYTES);
+    if ((lane & 3) == 0) {
+      ml_s[w][lane >> 2] = make_float2(m[0], l[0]);
+      ml_s[w][(lane >> 2) + 8] = make_float2(m[1], l[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(o_s + (w * 16 + (lane >> 2) + 8 * h) * DP + i * 8 + (lane & 3) * 2) =
+            make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    __syncthreads();
+    for (int x = threadIdx.x; x < n_rows * (DP / 2); x += 128) {
+      const int r = x / (DP / 2), d = x % (DP / 2) * 2;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) mm = fmaxf(mm, ml_s[y][r].x);
+      const float bs = mm == -INFINITY ? 0.0f : mm;
+      float ll = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float f = exp2f(ml_s[y][r].x - bs);
+        const float2 v = *reinterpret_cast<const float2*>(o_s + (y * 16 + r) * DP + d);
+        ll += f * ml_s[y][r].y;
+        o0 += f * v.x;
+        o1 += f * v.y;
+      }
+      if (d >= hd) continue;
+      const int rr = r0 + r;
+      const long long row = static_cast<long long>(e.t0 + rr / rep) * a.n_heads + kvh * rep + rr % rep;
+      const bool sees = e.row >= 0 && (pre || e.len - e.nq + rr / rep + 1 > 0);
+      if (whole) {
+        store_out<T>(a, row * hd + d, o0, o1, ll, sees);
+      } else {
+        *reinterpret_cast<float2*>(a.part_o + (part + row) * hd + d) = make_float2(o0, o1);
+        if (d == 0) a.part_ml[part + row] = make_float2(mm, ll);
+      }
+    }
+  }
+}
+
+// Join the parts of each (token, head): a warp a row, lane x has elements 4 x ... and 4 x + 128 ...
+template <typename T>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+  pdl_enter_grid();
+  const int lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= static_cast<long long>(a.n_tokens) * a.n_heads) return;
+  const int t = static_cast<int>(row / a.n_heads), hd = a.c.hd;
+  int i = t;
+  if (a.q_start != nullptr) {  // the last entry that starts at or before t
+    int lo = 0, up = a.n_batch;
+    while (up - lo > 1) {
+      const int mid = (lo + up) / 2;
+      if (a.q_start[mid] <= t) lo = mid;
+      else up = mid;
+    }
+    i = lo;
+  }
+  const int shared = shared_of(a);
+  const Entry e = entry_of(a, i, shared);
+  const bool sees = e.row >= 0 && t >= e.t0 && t < e.t0 + e.nq && e.len - e.nq + (t - e.t0) + 1 > 0;
+  int n_pre = 0, n_own = 0;
+  if (sees) {
+    if (e.shares) n_pre = cut_of(0, shared, a.n_pre).used;
+    n_own = cut_of(e.start, e.len, a.n_own).used;
+  }
+  const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
+  const int n = n_pre + n_own;
+  // part x < n: slots 0 .. n_pre - 1, then a.n_pre ...
+  auto slot_of = [&](int x) { return static_cast<long long>(x < n_pre ? x : a.n_pre + x - n_pre) * rows + row; };
+  float top = -INFINITY;
+  for (int x = lane; x < n; x += 32) top = fmaxf(top, a.part_ml[slot_of(x)].x);
+#pragma unroll
+  for (int y = 16; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, y));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int x = 0; x < n; ++x) {
+    const float2 ml = a.part_ml[slot_of(x)];
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing seen: its sums are not written
+    const float f = exp2f(ml.x - base);
+    l += f * ml.y;
+    const float* src = a.part_o + slot_of(x) * hd;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int d = lane * 4 + k * 128;
+      if (d < hd) {
+        const float4 v = *reinterpret_cast<const float4*>(src + d);
+        o[4 * k] += f * v.x;
+        o[4 * k + 1] += f * v.y;
+        o[4 * k + 2] += f * v.z;
+        o[4 * k + 3] += f * v.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = lane * 4 + k * 128;
+    if (d < hd) {
+      store_out<T>(a, row * hd + d, o[4 * k], o[4 * k + 1], l, sees);
+      store_out<T>(a, row * hd + d + 2, o[4 * k + 2], o[4 * k + 3], l, sees);
+    }
+  }
+}
+
+// How the work is divided: rows a block, and the parts of the prefix and of a sequence's own positions.
+struct AttnPlan {
+  int pre_wm, own_wm;
+  int pre_blocks, own_blocks;
+  int n_pre, n_own;
+};
+
+AttnPlan plan_of(int n_kv, bool ragged, int n_batch, int n_tokens, int n_heads, int shared_len, int max_len) {
+  AttnPlan p{};
+  const int sms = api_device_info().sm_count > 0 ? api_device_info().sm_count : 148;
+  const int rep = n_heads / n_kv;
+  const long long rows = static_cast<long long>(n_tokens) * rep;
+  p.own_wm = rows <= 16LL * n_batch ? 1 : 4;
+  const int own_rows = 16 * p.own_wm;
+  p.own_blocks = static_cast<int>(ragged ? (rows + own_rows - 1) / own_rows + n_batch
+                                         : static_cast<long long>(n_batch) * ((rep + own_rows - 1) / own_rows));
+  shared_len = std::max(0, std::min(shared_len, max_len));
+  const int own_tiles = (std::max(0, max_len - shared_len) + TILE - 1) / TILE + 1;
+  // two blocks an SM: enough parts for two rounds of them, none shorter than two tiles
+  const long long target = 4LL * sms;
+  const long long own_n = (target + static_cast<long long>(p.own_blocks) * n_kv - 1) / (static_cast<long long>(p.own_blocks) * n_kv);
+  p.n_own = static_cast<int>(std::max(1LL, std::min({own_n, static_cast<long long>((own_tiles + 1) / 2), static_cast<long long>(MAX_SLOTS)})));
+  if (shared_len > 0) {
+    p.pre_wm = rows <= 16 ? 1 : 4;
+    p.pre_blocks = static_cast<int>((rows + 16 * p.pre_wm - 1) / (16 * p.pre_wm));
+    const int tiles = (shared_len + TILE - 1) / TILE;
+    const long long n = 2LL * sms / (static_cast<long long>(p.pre_blocks) * n_kv);
+    p.n_pre = static_cast<int>(std::max(1LL, std::min({n, static_cast<long long>((tiles + 1) / 2), static_cast<long long>(MAX_SLOTS)})));
+  }
+  return p;
+}
+
+size_t work_bytes(const AttnPlan& p, int n_tokens, int n_heads, int hd) {
+  const int slots = p.n_pre + p.n_own;
+  if (slots <= 1) return 256;
+  return static_cast<size_t>(slots) * n_tokens * n_heads * (static_cast<size_t>(hd) * 4 + 8) + 256;
+}
+
+template <typename T, int DP, int WM>
+cudaError_t launch_rows_as(const AttnArgs& a, int blocks, int splits, int pre, cudaStream_t st) {
+  using L = RowsLayout<DP, WM>;
+  static const cudaError_t set =
+      cudaFuncSetAttribute(attn_rows_kernel<T, DP, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
+  if (set != cudaSuccess) return set;
+  return launch_dependent(attn_rows_kernel<T, DP, WM>, dim3(blocks, a.c.n_kv, splits), dim3(128), L::ALLOC, st, a, pre);
+}
+
+template <typename T>
+cudaError_t launch_rows(const AttnArgs& a, int wm, int blocks, int splits, int pre, cudaStream_t st) {
+  if (wm == 1)
+    return a.c.hd <= 64    ? launch_rows_as<T, 64, 1>(a, blocks, splits, pre, st)
+           : a.c.hd <= 128 ? launch_rows_as<T, 128, 1>(a, blocks, splits, pre, st)
+                           : launch_rows_as<T, 256, 1>(a, blocks, splits, pre, st);
+  return a.c.hd <= 64    ? launch_rows_as<T, 64, 4>(a, blocks, splits, pre, st)
+         : a.c.hd <= 128 ? launch_rows_as<T, 128, 4>(a, blocks, splits, pre, st)
+                         : launch_rows_as<T, 256, 4>(a, blocks, splits, pre, st);
+}
+
+template <typename T>
+cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
+  if (p.n_pre > 0) {
+    const cudaError_t e = launch_rows<T>(a, p.pre_wm, p.pre_blocks, p.n_pre, 1, st);
+    if (e != cudaSuccess) return e;
+  }
+  const cudaError_t e = launch_rows<T>(a, p.own_wm, p.own_blocks, p.n_own, 0, st);
+  if (e != cudaSuccess || p.n_pre + p.n_own == 1) return e;
+  const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
+  return launch_dependent(attn_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, st, a);
+}
+
+}  // namespace
+}  // namespace ex
+
+extern "C" {
+
+size_t edgexpu_cuda_kv_attention_work_bytes(const edgexpu_cuda_kv_cache* cache, int n_batch, int n_tokens, int n_heads,
+                                            int shared_len, int max_len) {
+  if (cache == nullptr || cache->n_kv < 1 || n_heads < 1 || n_heads % cache->n_kv != 0 || n_batch < 1 || n_tokens < 1 ||
+      max_len < 1 || cache->head_dim < 1)
+    return 0;
+  // one token each may come with q_start or without: the larger of the two divisions
+  const ex::AttnPlan p = ex::plan_of(cache->n_kv, true, n_batch, n_tokens, n_heads, shared_len, max_len);
+  const ex::AttnPlan u = ex::plan_of(cache->n_kv, false, n_batch, n_tokens, n_heads, shared_len, max_len);
+  return std::max(ex::work_bytes(p, n_tokens, n_heads, cache->head_dim), ex::work_bytes(u, n_tokens, n_heads, cache->head_dim));
+}
+
+int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer, const void* q, const int32_t* seqs,
+                                  const int32_t* q_start, int n_batch, int n_tokens, int n_heads, int shared_seq,
+                                  int shared_len, int max_len, float scale, void* out, uint32_t out_type, void* work,
+                                  size_t work_size, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  if (!ex::api_ready(nullptr, 0)) return 0;
+  ex::AttnArgs a{};
+  if (!ex::kv_view(cache, "kv_attention", &a.c)) return 0;
+  if (n_batch < 0 || n_tokens < 0 || n_heads < 1 || n_heads % a.c.n_kv != 0 || layer < 0 || layer >= a.c.n_layers)
+    return ex::api_fail(nullptr, 0, "kv_attention: %d entries, %d tokens, %d heads over %d, layer %d of %d", n_batch, n_tokens,
+                        n_heads, a.c.n_kv, layer, a.c.n_layers);
+  if (n_tokens == 0) return 1;
+  if (q == nullptr || seqs == nullptr || out == nullptr || n_batch < 1 || (q_start == nullptr && n_tokens != n_batch))
+    return ex::api_fail(nullptr, 0, "kv_attention: invalid arguments (%d tokens of %d entries)", n_tokens, n_batch);
+  if (out_type != ex::TYPE_F32 && out_type != cache->type)
+    return ex::api_fail(nullptr, 0, "kv_attention: output type %u (F32, or the cache's %u)", out_type, cache->type);
+  if (shared_len > 0 && (shared_seq < 0 || shared_seq >= a.c.n_seqs))
+    return ex::api_fail(nullptr, 0, "kv_attention: shared sequence %d of %d", shared_seq, a.c.n_seqs);
+  if (max_len < 1) return ex::api_fail(nullptr, 0, "kv_attention: max_len %d", max_len);
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
+    return ex::api_fail(nullptr, 0, "kv_attention: q and out must be 16-byte aligned");
+  const ex::AttnPlan p = ex::plan_of(a.c.n_kv, q_start != nullptr, n_batch, n_tokens, n_heads, shared_len, max_len);
+  const size_t need = ex::work_bytes(p, n_tokens, n_heads, a.c.hd);
+  const long long rows = static_cast<long long>(n_tokens) * n_heads;
+  if (rows > INT_MAX || p.own_blocks < 1) return ex::api_fail(nullptr, 0, "kv_attention: %d tokens in one call", n_tokens);
+  if (work == nullptr || work_size < need || (reinterpret_cast<uintptr_t>(work) & 255) != 0)
+    return ex::api_fail(nullptr, 0, "kv_attention: work memory of %zu bytes, 256-byte aligned, is needed (got %zu)", need,
+                        work == nullptr ? static_cast<size_t>(0) : work_size);
+  a.layer_off = layer * a.c.layer_stride;
+  a.q = static_cast<const uint16_t*>(q);
+  a.seqs = seqs;
+  a.q_start = q_start;
+  a.n_batch = n_batch;
+  a.n_tokens = n_tokens;
+  a.n_heads = n_heads;
+  a.rep = n_heads / a.c.n_kv;
+  a.shared_seq = shared_len > 0 ? shared_seq : 0;
+  a.shared_len = std::max(0, std::min(shared_len, max_len));
+  a.scale = scale * 1.4426950408889634f;
+  a.n_pre = p.n_pre;
+  a.n_own = p.n_own;
+  const int slots = p.n_pre + p.n_own;
+  a.part_ml = static_cast<float2*>(work);
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + (static_cast<size_t>(slots) * rows * 8 + 15) / 16 * 16);
+  a.out = out;
+  a.out_f32 = out_type == ex::TYPE_F32;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cache->type == ex::TYPE_F16 ? ex::launch_attention_as<__half>(a, p, st)
+                                                    : ex::launch_attention_as<__nv_bfloat16>(a, p, st);
+  if (e != cudaSuccess) return ex::api_fail(nullptr, 0, "kv_attention: %s", cudaGetErrorString(e));
+  return 1;
+}
+
+}  // extern "C"

@@ -1,0 +1,641 @@
+// kvcache.cu -- a key/value cache in pages that many sequences share: taking, sharing, copying,
+// packing and giving back pages, and the pass that norms, rotates and stores the heads of new tokens.
+//
+// State.  table[s][i] names the page of positions i * page_size ... of sequence s, refs[p] counts the
+// rows that name page p, and a page with refs 0 is free.  All of it lives on the device, so a decode
+// loop that takes pages can be a CUDA graph; the price is that finding free pages is a scan of refs.
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cstring>
+#include <mutex>
+
+#include "capi_internal.h"
+#include "kv.cuh"
+
+namespace ex {
+namespace {
+
+constexpr int APPEND_MAX = 4096;  // entries of one append: four a thread of the one block that plans it
+constexpr int PLAN_THREADS = 1024;
+constexpr int WORK_HEAD = 16;     // ints: [0] the copies or moves that a plan found
+
+// work: head | owner[n_seqs] | count[n_pages] | last[n_pages] | list[n_pages] | jobs[3 * n_seqs].
+// A packing keeps its sources in count, its destinations in last and every page's new index in list.
+struct Work {
+  int32_t *head, *owner, *count, *last, *list, *jobs;
+};
+__host__ __device__ __forceinline__ Work work_of(const KvView& c) {
+  Work w;
+  w.head = c.work;
+  w.owner = w.head + WORK_HEAD;
+  w.count = w.owner + c.n_seqs;
+  w.last = w.count + c.n_pages;
+  w.list = w.last + c.n_pages;
+  w.jobs = w.list + c.n_pages;
+  return w;
+}
+
+// ---- giving back and sharing ------------------------------------------------------------------------
+
+// One block a batch entry.  A page leaves its row by an exchange, so an entry that comes twice gives
+// it back once.
+__global__ void __launch_bounds__(128) kv_free_kernel(const KvView c, const int32_t* seqs, const int32_t* keep) {
+  pdl_enter_grid();
+  const int s = seqs[blockIdx.x];
+  if (s < 0) return;
+  if (s >= c.n_seqs) {
+    if (threadIdx.x == 0) atomicOr(c.status, ST_BAD_CACHE);
+    return;
+  }
+  const int len = max(0, c.lens[s]);
+  const int kept = keep != nullptr ? min(max(0, keep[blockIdx.x]), len) : 0;
+  const int end = min(kv_pages_of(c, len), c.max_pages);
+  int32_t* row = c.table + static_cast<long long>(s) * c.max_pages;
+  for (int i = kv_pages_of(c, kept) + threadIdx.x; i < end; i += blockDim.x) {
+    const int p = atomicExch(&row[i], -1);
+    if (p >= 0 && p < c.n_pages)
+      atomicSub(&c.refs[p], 1);
+    else if (p >= c.n_pages)
+      atomicOr(c.status, ST_BAD_CACHE);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) atomicMin(&c.lens[s], kept);
+}
+
+// One block a batch entry.  An entry is refused for what the batch alone shows (a destination that
+// comes earlier too, a source that is a destination) or for a destination that holds tokens; no other
+// entry writes what it reads then.
+__global__ void __launch_bounds__(256) kv_fork_kernel(const KvView c, const int32_t* src, const int32_t* dst, int n) {
+  pdl_enter_grid();
+  const int b = blockIdx.x, s = src[b], d = dst[b];
+  if (d < 0) return;
+  int bad = s < 0 || s >= c.n_seqs || d >= c.n_seqs;
+  for (int j = threadIdx.x; j < n && !bad; j += blockDim.x) bad = (j < b && dst[j] == d) || dst[j] == s;
+  bad = __syncthreads_or(bad);
+  if (!bad) bad = c.lens[d] != 0;
+  if (bad) {
+    if (threadIdx.x == 0) atomicOr(c.status, ST_BAD_CACHE);
+    return;
+  }
+  __syncthreads();  // every thread has read lens[d]
+  const int len = max(0, c.lens[s]), pages = min(kv_pages_of(c, len), c.max_pages);
+  const int32_t* from = c.table + static_cast<long long>(s) * c.max_pages;
+  int32_t* to = c.table + static_cast<long long>(d) * c.max_pages;
+  for (int i = threadIdx.x; i < pages; i += blockDim.x) {
+    const int p = from[i];
+    to[i] = p;
+    if (p >= 0 && p < c.n_pages)
+      atomicAdd(&c.refs[p], 1);
+    else
+      atomicOr(c.status, ST_BAD_CACHE);
+  }
+  if (threadIdx.x == 0) c.lens[d] = len;
+}
+
+// ---- block-wide scans ---------------------------------------------------------------------------------
+
+// Exclusive sum of v over the block's threads in order; *total = the whole.  red: 33 ints.
+__device__ __forceinline__ int block_scan(int v, int* red, int* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) red[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    int t = lane < nw ? red[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, t, o);
+      if (lane >= o) t += y;
+    }
+    red[lane] = t;
+  }
+  __syncthreads();
+  const int r = x - v + (w > 0 ? red[w - 1] : 0);
+  *total = red[nw - 1];
+  __syncthreads();
+  return r;
+}
+
+// The indices i in [from, to) with (refs[i] > 0) == live, ascending, into list[at ...) (list nullable);
+// stops once `most` are found.  Returns how many of them there are up to where it stopped.  All
+// threads of the block call it.
+__device__ int find_pages(const int32_t* refs, int from, int to, bool live, int most, int32_t* list, int* red) {
+  constexpr int UN = 8;  // loads in flight a thread
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int found = 0;
+  for (int base = from; base < to && found < most; base += nw * 32 * UN) {
+    const int b = base + w * 32 * UN + lane;
+    uint32_t hit[UN];
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int i = b + u * 32;
+      const bool h = i < to && (refs[i] > 0) == live;
+      hit[u] = __ballot_sync(0xFFFFFFFFu, h);
+      mine += __popc(hit[u]);
+    }
+    int total;
+    // every lane of a warp carries the warp's count; the first one enters it into the scan
+    int off = block_scan(lane == 0 ? mine : 0, red, &total);
+    off = found + __shfl_sync(0xFFFFFFFFu, off, 0);
+    if (list != nullptr) {
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        if ((hit[u] >> lane) & 1u) list[off + __popc(hit[u] & ((1u << lane) - 1u))] = b + u * 32;
+        off += __popc(hit[u]);
+      }
+    }
+    found += total;
+  }
+  return found;
+}
+
+// ---- taking -------------------------------------------------------------------------------------------
+
+// One block: what each entry needs, the lowest free pages for it, and the last pages to be copied.
+// With 64 sequences it is bound by latency (a chain of dependent loads and block barriers).
+__global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvView c, const int32_t* seqs,
+                                                                      const int32_t* n_new, int n, int32_t* pos,
+                                                                      int32_t* missing) {
+  pdl_enter_grid();
+  constexpr int PER = APPEND_MAX / PLAN_THREADS;
+  __shared__ int s_first[APPEND_MAX], s_off[APPEND_MAX + 1];  // an entry's first new column, its first place in the list
+  __shared__ int red[33];
+  __shared__ int n_jobs;
+  const Work w = work_of(c);
+  if (threadIdx.x == 0) n_jobs = 0;
+  // a sequence belongs to the first entry that names it
+  for (int b = threadIdx.x; b < n; b += blockDim.x)
+    if (seqs[b] >= 0 && seqs[b] < c.n_seqs) w.owner[seqs[b]] = INT_MAX;
+  __syncthreads();
+  for (int b = threadIdx.x; b < n; b += blockDim.x)
+    if (seqs[b] >= 0 && seqs[b] < c.n_seqs) atomicMin(&w.owner[seqs[b]], b);
+  __syncthreads();
+  // entries 4 * thread ..., so that a scan over threads is a scan over the batch
+  int len[PER], add[PER], tail[PER];  // tail: the page that holds the last tokens, when it has room; else -1
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int b = threadIdx.x * PER + e;
+    len[e] = add[e] = tail[e] = -1;
+    if (b >= n || seqs[b] < 0) continue;
+    const int s = seqs[b];
+    bool ok = s < c.n_seqs && w.owner[s] == b;
+    if (ok) {
+      const int held = c.lens[s], more = n_new[b];
+      ok = held >= 0 && more >= 0 && static_cast<long long>(held) + more <= (static_cast<long long>(c.max_pages) << c.ps_shift);
+      if (ok) {
+        len[e] = held;
+        add[e] = more;
+        if ((held & ((1 << c.ps_shift) - 1)) != 0 && more > 0) {
+          tail[e] = c.table[static_cast<long long>(s) * c.max_pages + (held >> c.ps_shift)];
+          if (tail[e] < 0 || tail[e] >= c.n_pages) {
+            ok = false;
+            len[e] = add[e] = tail[e] = -1;
+          }
+        }
+      }
+    }
+    if (!ok) atomicOr(c.status, ST_BAD_CACHE);
+    if (tail[e] >= 0) {
+      w.count[tail[e]] = 0;
+      w.last[tail[e]] = -1;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < PER; ++e)
+    if (tail[e] >= 0) {
+      atomicAdd(&w.count[tail[e]], 1);
+      atomicMax(&w.last[tail[e]], static_cast<int>(threadIdx.x) * PER + e);
+    }
+  __syncthreads();
+  int need = 0, want[PER];
+  bool split[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int b = threadIdx.x * PER + e;
+    split[e] = false;
+    want[e] = 0;
+    if (tail[e] >= 0) {
+      const int r = c.refs[tail[e]];
+      split[e] = r > 1 && !(w.count[tail[e]] >= r && w.last[tail[e]] == b);
+    }
+    if (add[e] >= 0) {
+      s_first[b] = kv_pages_of(c, len[e]) - (split[e] ? 1 : 0);
+      want[e] = kv_pages_of(c, len[e] + add[e]) - s_first[b];
+      need += want[e];
+    }
+  }
+  int total;
+  int off = block_scan(need, red, &total);
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int b = threadIdx.x * PER + e;
+    if (b < n) s_off[b] = off;
+    off += want[e];
+  }
+  if (threadIdx.x == 0) s_off[n] = total;
+  const int found = total > 0 ? find_pages(c.refs, 0, c.n_pages, false, total, w.list, red) : 0;
+  const bool fits = found >= total;
+  __syncthreads();
+  if (fits) {  // a warp an entry: its pages into its row
+    const int lane = threadIdx.x & 31;
+    for (int b = threadIdx.x >> 5; b < n; b += blockDim.x >> 5) {
+      const int at = s_off[b], take = s_off[b + 1] - at;
+      if (take == 0) continue;
+      int32_t* row = c.table + static_cast<long long>(seqs[b]) * c.max_pages + s_first[b];
+      for (int i = lane; i < take; i += 32) {
+        const int p = w.list[at + i];
+        row[i] = p;
+        c.refs[p] = 1;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int b = threadIdx.x * PER + e;
+    if (b >= n) continue;
+    const bool done = fits && add[e] >= 0;
+    if (pos != nullptr) pos[b] = done ? len[e] : -1;
+    if (!done) continue;
+    c.lens[seqs[b]] = len[e] + add[e];
+    if (split[e]) {
+      atomicSub(&c.refs[tail[e]], 1);
+      const int j = atomicAdd(&n_jobs, 1);
+      w.jobs[3 * j] = tail[e];
+      w.jobs[3 * j + 1] = w.list[s_off[b]];
+      w.jobs[3 * j + 2] = len[e] & ((1 << c.ps_shift) - 1);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    w.head[0] = n_jobs;
+    if (missing != nullptr)
+      *missing = fits ? 0 : total - found;
+    else if (!fits)
+      atomicOr(c.status, ST_NO_PAGES);
+  }
+}
+
+// ---- moving -------------------------------------------------------------------------------------------
+
+constexpr int PIECE = 4096;  // bytes a warp copies at once: eight 16-byte loads a thread in flight
+
+// Pages (or their first tokens) from src to dst, in every layer, in k and v.  The unit of work is a
+// PIECE of one head of one page of one layer of one pool; warps take them in turn.  Bound by HBM.
+//   stride 1: job i is src[i] -> dst[i], all tokens; stride 3: jobs[3i], jobs[3i + 1], jobs[3i + 2] tokens.
+//   n_dev: the number of jobs, on the device; else n.
+//   remap: afterwards table entries p >= *n_dev_live become remap[p] (a packing).
+struct MoveArgs {
+  const int32_t* src;
+  const int32_t* dst;
+  int stride;
+  int n;
+  const int32_t* n_dev;
+  const int32_t* n_live;
+  const int32_t* remap;
+};
+
+__global__ void __launch_bounds__(256) kv_move_kernel(const KvView c, const MoveArgs a) {
+  pdl_enter_grid();
+  const int lane = threadIdx.x & 31;
+  const long long warp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const long long n_warps = (static_cast<long long>(gridDim.x) * blockDim.x) >> 5;
+  const int n = a.n_dev != nullptr ? *a.n_dev : a.n;
+  const int ps = 1 << c.ps_shift, head_bytes = ps * c.hd * 2;
+  const int pieces = (head_bytes + PIECE - 1) / PIECE;
+  const long long per_job = static_cast<long long>(c.n_layers) * 2 * c.n_kv * pieces;
+  for (long long u = warp; u < n * per_job; u += n_warps) {
+    const int job = static_cast<int>(u / per_job);
+    int r = static_cast<int>(u - job * per_job);
+    const int piece = r % pieces;
+    r /= pieces;
+    const int h = r % c.n_kv;
+    r /= c.n_kv;
+    const int layer = r >> 1;
+    uint16_t* pool = (r & 1) != 0 ? c.v : c.k;
+    const int from = a.src[job * a.stride], to = a.dst[job * a.stride];
+    if (from < 0 || from >= c.n_pages || to < 0 || to >= c.n_pages) {
+      if (lane == 0) atomicOr(c.status, ST_BAD_CACHE);
+      continue;
+    }
+    const int bytes = a.stride == 3 ? a.src[job * 3 + 2] * c.hd * 2 : head_bytes;
+    uint16_t* base = pool + layer * c.layer_stride + static_cast<long long>(h) * ps * c.hd;
+    const uint4* s = reinterpret_cast<const uint4*>(base + from * c.page_stride);
+    uint4* d = reinterpret_cast<uint4*>(base + to * c.page_stride);
+    const int first = piece * (PIECE / 16) + lane, end = min(bytes, (piece + 1) * PIECE) / 16;
+    uint4 x[PIECE / 512];
+#pragma unroll
+    for (int i = 0; i < PIECE / 512; ++i)
+      if (first + i * 32 < end) x[i] = __ldcs(s + first + i * 32);
+#pragma unroll
+    for (int i = 0; i < PIECE / 512; ++i)
+      if (first + i * 32 < end) __stcs(d + first + i * 32, x[i]);
+  }
+  if (a.remap != nullptr) {
+    const int live = *a.n_live;
+    const long long cells = static_cast<long long>(c.n_seqs) * c.max_pages, step = static_cast<long long>(gridDim.x) * blockDim.x;
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < cells; i += step) {
+      const int p = c.table[i];
+      if (p >= live) {
+        if (p < c.n_pages)
+          c.table[i] = a.remap[p];
+        else
+          atomicOr(c.status, ST_BAD_CACHE);
+      }
+    }
+  }
+}
+
+// One block: the pages in use at or above their number L, the free ones below it, and the reference
+// counts after the moves.
+__global__ void __launch_bounds__(PLAN_THREADS) kv_compact_plan_kernel(const KvView c, int32_t* n_live) {
+  pdl_enter_grid();
+  __shared__ int red[33];
+  const Work w = work_of(c);
+  const int live = find_pages(c.refs, 0, c.n_pages, true, INT_MAX, nullptr, red);
+  const int moves = find_pages(c.refs, live, c.n_pages, true, INT_MAX, w.count, red);
+  find_pages(c.refs, 0, live, false, INT_MAX, w.last, red);
+  for (int p = live + threadIdx.x; p < c.n_pages; p += blockDim.x) w.list[p] = p;
+  __syncthreads();
+  for (int i = threadIdx.x; i < moves; i += blockDim.x) {
+    const int s = w.count[i], d = w.last[i];
+    w.list[s] = d;
+    c.refs[d] = c.refs[s];
+    c.refs[s] = 0;
+  }
+  if (threadIdx.x == 0) {
+    w.head[0] = moves;
+    w.head[1] = live;
+    if (n_live != nullptr) *n_live = live;
+  }
+}
+
+cudaError_t launch_move(const KvView& c, const MoveArgs& a, long long jobs_at_most, cudaStream_t st) {
+  const long long pieces = (static_cast<long long>(2 << c.ps_shift) * c.hd + PIECE - 1) / PIECE;
+  const long long warps = jobs_at_most * c.n_layers * 2 * c.n_kv * pieces;
+  long long blocks = (warps + 7) / 8;
+  const long long most = 8LL * api_device_info().sm_count;  // 2048 threads an SM
+  if (blocks > most) blocks = most;
+  if (blocks < 1) blocks = 1;
+  return launch_dependent(kv_move_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, c, a);
+}
+
+// ---- norm, rotation and store of new tokens' heads ----------------------------------------------------
+
+struct QkArgs {
+  const float *q, *k, *v;
+  long long qs, ks, vs;
+  int n_tokens, n_heads, layer;
+  const float *qw, *kw;
+  float eps;
+  const float* rope;
+  int rope_positions, rot, halves;
+  const int32_t *seqs, *pos;
+  uint16_t* q_out;
+};
+
+constexpr int QK_WARPS = 8;
+
+// A warp a head of a token: its elements as float4 (lane, lane + 32), the sum of squares in fp32 over
+// the warp, the normed row through shared memory so that either pairing finds its partners, and one
+// 8-byte store per four elements.  Bound by HBM: 4 bytes read and 2 written an element.
+template <typename T>
+__global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvView c, const QkArgs a) {
+  pdl_enter_grid();
+  __shared__ __align__(16) float rows[QK_WARPS][256];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int per_token = a.n_heads + 2 * c.n_kv;
+  const long long item = static_cast<long long>(blockIdx.x) * QK_WARPS + w;
+  if (item >= static_cast<long long>(a.n_tokens) * per_token) return;
+  const int t = static_cast<int>(item / per_token), h = static_cast<int>(item % per_token);
+  const int kind = h < a.n_heads ? 0 : h < a.n_heads + c.n_kv ? 1 : 2;  // q, k, v
+  const int hh = kind == 0 ? h : kind == 1 ? h - a.n_heads : h - a.n_heads - c.n_kv;
+  const int s = a.seqs[t], p = a.pos[t], nv = c.hd / 4;
+  bool live = s >= 0 && p >= 0;
+  int page = -1;
+  if (live) {
+    if (s < c.n_seqs && (p >> c.ps_shift) < c.max_pages && (a.rope == nullptr || p < a.rope_positions))
+      page = c.table[static_cast<long long>(s) * c.max_pages + (p >> c.ps_shift)];
+    if (page < 0 || page >= c.n_pages) {
+      live = false;
+      if (lane == 0) atomicOr(c.status, ST_BAD_CACHE);
+    }
+  }
+  uint16_t* dst;
+  if (kind == 0) {
+    dst = a.q_out + (static_cast<long long>(t) * a.n_heads + hh) * c.hd;
+  } else {
+    if (!live) return;
+    dst = (kind == 1 ? c.k : c.v) + a.layer * c.layer_stride + page * c.page_stride +
+          ((static_cast<long long>(hh) << c.ps_shift) + (p & ((1 << c.ps_shift) - 1))) * c.hd;
+  }
+  if (!live) {
+    for (int i = lane; i < nv; i += 32) reinterpret_cast<uint2*>(dst)[i] = make_uint2(0u, 0u);
+    return;
+  }
+  const float* x = kind == 0 ? a.q + t * a.qs : kind == 1 ? a.k + t * a.ks : a.v + t * a.vs;
+  const float4* x4 = reinterpret_cast<const float4*>(x + static_cast<long long>(hh) * c.hd);
+  float4 e[2];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + i * 32;
+    e[i] = j < nv ? x4[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    ss += e[i].x * e[i].x + e[i].y * e[i].y + e[i].z * e[i].z + e[i].w * e[i].w;
+  }
+  if (kind < 2) {
+    const float* wt = kind == 0 ? a.qw : a.kw;
+    if (wt != nullptr) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+      const float r = 1.0f / sqrtf(ss / static_cast<float>(c.hd) + a.eps);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = lane + i * 32;
+        if (j < nv) {
+          e[i].x = e[i].x * r * wt[4 * j];
+          e[i].y = e[i].y * r * wt[4 * j + 1];
+          e[i].z = e[i].z * r * wt[4 * j + 2];
+          e[i].w = e[i].w * r * wt[4 * j + 3];
+        }
+      }
+    }
+    if (a.rope != nullptr) {
+      float* row = rows[w];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane + i * 32 < nv) reinterpret_cast<float4*>(row)[lane + i * 32] = e[i];
+      __syncwarp();
+      const float* cs = a.rope + static_cast<long long>(p) * a.rot;
+      const int half = a.rot / 2;
+      for (int j = lane; j < half; j += 32) {
+        const int i0 = a.halves ? j : 2 * j, i1 = a.halves ? j + half : 2 * j + 1;
+        const float cc = cs[2 * j], sn = cs[2 * j + 1], y0 = row[i0], y1 = row[i1];
+        row[i0] = y0 * cc - y1 * sn;
+        row[i1] = y0 * sn + y1 * cc;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane + i * 32 < nv) e[i] = reinterpret_cast<float4*>(row)[lane + i * 32];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + i * 32 < nv)
+      reinterpret_cast<uint2*>(dst)[lane + i * 32] = make_uint2(pack16<T>(e[i].x, e[i].y), pack16<T>(e[i].z, e[i].w));
+}
+
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+}  // namespace
+
+int kv_view(const edgexpu_cuda_kv_cache* c, const char* who, KvView* view) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr || c->table == nullptr || c->lens == nullptr || c->refs == nullptr)
+    return api_fail(nullptr, 0, "%s: the cache or one of its arrays is NULL", who);
+  if (c->type != TYPE_F16 && c->type != TYPE_BF16)
+    return api_fail(nullptr, 0, "%s: cache type %u (F16 and BF16 are supported)", who, c->type);
+  int shift = 0;
+  while (shift < 8 && (1 << shift) < c->page_size) ++shift;
+  if (c->page_size < 16 || (1 << shift) != c->page_size)
+    return api_fail(nullptr, 0, "%s: page size %d (16, 32, 64, 128 or 256)", who, c->page_size);
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 != 0)
+    return api_fail(nullptr, 0, "%s: head_dim %d (a multiple of 8, 256 at most)", who, c->head_dim);
+  if (c->n_layers < 1 || c->n_pages < 1 || c->n_kv < 1 || c->n_kv > 65535 || c->n_seqs < 1 || c->max_pages < 1)
+    return api_fail(nullptr, 0, "%s: layers, pages, heads, sequences and columns must be positive", who);
+  if ((static_cast<long long>(c->max_pages) << shift) > INT_MAX)
+    return api_fail(nullptr, 0, "%s: a row of %d pages holds more than 2^31 - 1 positions", who, c->max_pages);
+  const long long page = static_cast<long long>(c->n_kv) * c->page_size * c->head_dim;
+  if (c->page_stride < page || c->page_stride % 8 != 0 || c->layer_stride < 0 || c->layer_stride % 8 != 0)
+    return api_fail(nullptr, 0, "%s: strides %lld, %lld (multiples of 8; a page has %lld elements)", who,
+                    static_cast<long long>(c->layer_stride), static_cast<long long>(c->page_stride), page);
+  if (!aligned(c->k, 16) || !aligned(c->v, 16)) return api_fail(nullptr, 0, "%s: k and v must be 16-byte aligned", who);
+  *view = KvView{static_cast<uint16_t*>(c->k), static_cast<uint16_t*>(c->v), c->layer_stride, c->page_stride, c->n_layers,
+                 c->n_pages, shift, c->n_kv, c->head_dim, c->n_seqs, c->max_pages, c->table, c->lens, c->refs, c->work,
+                 api_status_word()};
+  return 1;
+}
+
+namespace {
+
+// What every page call checks: a bound device, a cache, its scratch where the call needs it, a batch.
+int page_call(const edgexpu_cuda_kv_cache* c, const char* who, bool scratch, int n, bool arrays, KvView* view) {
+  if (!api_ready(nullptr, 0) || !kv_view(c, who, view)) return 0;
+  if (scratch && c->work == nullptr) return api_fail(nullptr, 0, "%s: the cache has no work memory", who);
+  if (n < 0 || !arrays) return api_fail(nullptr, 0, "%s: invalid arguments", who);
+  return 1;
+}
+
+int launched(cudaError_t e, const char* who) {
+  return e == cudaSuccess ? 1 : api_fail(nullptr, 0, "%s: %s", who, cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace ex
+
+extern "C" {
+
+size_t edgexpu_cuda_kv_work_bytes(int n_pages, int n_seqs) {
+  if (n_pages < 1 || n_seqs < 1) return 0;
+  return (static_cast<size_t>(ex::WORK_HEAD) + 4 * static_cast<size_t>(n_seqs) + 3 * static_cast<size_t>(n_pages)) * 4;
+}
+
+int edgexpu_cuda_kv_append_dev(const edgexpu_cuda_kv_cache* cache, const int32_t* seqs, const int32_t* n_new, int n,
+                               int32_t* pos, int32_t* missing, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  ex::KvView c;
+  if (!ex::page_call(cache, "kv_append", true, n, n == 0 || (seqs != nullptr && n_new != nullptr), &c)) return 0;
+  if (n > ex::APPEND_MAX) return ex::api_fail(nullptr, 0, "kv_append: %d entries (at most %d)", n, ex::APPEND_MAX);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = ex::launch_dependent(ex::kv_append_plan_kernel, dim3(1), dim3(ex::PLAN_THREADS), 0, st, c, seqs, n_new, n, pos, missing);
+  if (e == cudaSuccess && n > 0) {
+    const ex::Work w = ex::work_of(c);
+    const ex::MoveArgs a{w.jobs, w.jobs + 1, 3, 0, w.head, nullptr, nullptr};
+    e = ex::launch_move(c, a, n, st);
+  }
+  return ex::launched(e, "kv_append");
+}
+
+int edgexpu_cuda_kv_fork_dev(const edgexpu_cuda_kv_cache* cache, const int32_t* src, const int32_t* dst, int n, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  ex::KvView c;
+  if (!ex::page_call(cache, "kv_fork", false, n, n == 0 || (src != nullptr && dst != nullptr), &c)) return 0;
+  if (n == 0) return 1;
+  return ex::launched(ex::launch_dependent(ex::kv_fork_kernel, dim3(n), dim3(256), 0, static_cast<cudaStream_t>(stream), c, src, dst, n),
+                      "kv_fork");
+}
+
+int edgexpu_cuda_kv_free_dev(const edgexpu_cuda_kv_cache* cache, const int32_t* seqs, const int32_t* keep, int n, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  ex::KvView c;
+  if (!ex::page_call(cache, "kv_free", false, n, n == 0 || seqs != nullptr, &c)) return 0;
+  if (n == 0) return 1;
+  return ex::launched(ex::launch_dependent(ex::kv_free_kernel, dim3(n), dim3(128), 0, static_cast<cudaStream_t>(stream), c, seqs, keep),
+                      "kv_free");
+}
+
+int edgexpu_cuda_kv_copy_dev(const edgexpu_cuda_kv_cache* cache, const int32_t* src, const int32_t* dst, int n, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  ex::KvView c;
+  if (!ex::page_call(cache, "kv_copy", false, n, n == 0 || (src != nullptr && dst != nullptr), &c)) return 0;
+  if (n == 0) return 1;
+  const ex::MoveArgs a{src, dst, 1, n, nullptr, nullptr, nullptr};
+  return ex::launched(ex::launch_move(c, a, n, static_cast<cudaStream_t>(stream)), "kv_copy");
+}
+
+int edgexpu_cuda_kv_compact_dev(const edgexpu_cuda_kv_cache* cache, int32_t* n_live, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  ex::KvView c;
+  if (!ex::page_call(cache, "kv_compact", true, 0, true, &c)) return 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const ex::Work w = ex::work_of(c);
+  cudaError_t e = ex::launch_dependent(ex::kv_compact_plan_kernel, dim3(1), dim3(ex::PLAN_THREADS), 0, st, c, n_live);
+  const ex::MoveArgs a{w.count, w.last, 1, 0, w.head, w.head + 1, w.list};
+  if (e == cudaSuccess) e = ex::launch_move(c, a, c.n_pages, st);
+  return ex::launched(e, "kv_compact");
+}
+
+int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache* cache, int layer, const float* q, const float* k,
+                                  const float* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, int n_tokens,
+                                  int n_heads, const float* q_weight, const float* k_weight, float eps, const float* rope,
+                                  int rope_positions, int rope_dims, int rope_pairing, const int32_t* seqs,
+                                  const int32_t* pos, void* q_out, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(ex::api_mutex());
+  ex::KvView c;
+  if (!ex::page_call(cache, "qk_norm_rope", false, n_tokens,
+                     n_tokens == 0 || (q != nullptr && k != nullptr && v != nullptr && seqs != nullptr && pos != nullptr &&
+                                       q_out != nullptr),
+                     &c))
+    return 0;
+  if (layer < 0 || layer >= c.n_layers || n_heads < 1)
+    return ex::api_fail(nullptr, 0, "qk_norm_rope: layer %d of %d, %d heads", layer, c.n_layers, n_heads);
+  const int64_t qn = static_cast<int64_t>(n_heads) * c.hd, kn = static_cast<int64_t>(c.n_kv) * c.hd;
+  if (q_stride < qn || k_stride < kn || v_stride < kn || q_stride % 4 != 0 || k_stride % 4 != 0 || v_stride % 4 != 0 ||
+      !ex::aligned(q, 16) || !ex::aligned(k, 16) || !ex::aligned(v, 16) || !ex::aligned(q_out, 16))
+    return ex::api_fail(nullptr, 0, "qk_norm_rope: rows must be 16-byte aligned and at least %lld and %lld floats apart",
+                        static_cast<long long>(qn), static_cast<long long>(kn));
+  if (rope != nullptr && (rope_positions < 1 || rope_dims < 2 || rope_dims > c.hd || rope_dims % 2 != 0))
+    return ex::api_fail(nullptr, 0, "qk_norm_rope: a table of %d positions and %d dims for heads of %d", rope_positions, rope_dims, c.hd);
+  if (rope_pairing != EDGEXPU_CUDA_ROPE_ADJACENT && rope_pairing != EDGEXPU_CUDA_ROPE_HALVES)
+    return ex::api_fail(nullptr, 0, "qk_norm_rope: pairing %d", rope_pairing);
+  if (n_tokens == 0) return 1;
+  const long long items = static_cast<long long>(n_tokens) * (n_heads + 2LL * c.n_kv);
+  const long long blocks = (items + ex::QK_WARPS - 1) / ex::QK_WARPS;
+  if (blocks > INT_MAX) return ex::api_fail(nullptr, 0, "qk_norm_rope: %d tokens in one call", n_tokens);
+  const ex::QkArgs a{q, k, v, q_stride, k_stride, v_stride, n_tokens, n_heads, layer, q_weight, k_weight, eps, rope,
+                     rope_positions, rope_dims, rope_pairing == EDGEXPU_CUDA_ROPE_HALVES, seqs, pos,
+                     static_cast<uint16_t*>(q_out)};
+  auto kern = cache->type == ex::TYPE_F16 ? ex::qk_norm_rope_kernel<__half> : ex::qk_norm_rope_kernel<__nv_bfloat16>;
+  return ex::launched(ex::launch_dependent(kern, dim3(static_cast<unsigned>(blocks)), dim3(ex::QK_WARPS * 32), 0,
+                                           static_cast<cudaStream_t>(stream), c, a),
+                      "qk_norm_rope");
+}
+
+}  // extern "C"

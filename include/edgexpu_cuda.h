@@ -25,6 +25,7 @@
  *   edgexpu_cuda_dequantize_row       edgexpu_gguf_dequantize_row       include/edgexpu/gguf_quant.h:50-58
  *   edgexpu_cuda_dequantize_rows_dev  the token-embedding gather of embedding_row src/native.c:428-443
  *                                     (a batch of rows, device buffers)
+ *   edgexpu_cuda_kv_*, _qk_norm_rope_dev   none: a cache of pages for many sequences, and its attention
  *
  * Weight handles: edgexpu_cuda_upload_weight returns a device address (typed const uint8_t *)
  * that callers keep in edgexpu_qweight.data (include/edgexpu/native.h:23-28) in place of the
@@ -58,6 +59,8 @@ extern "C" {
 #define EDGEXPU_CUDA_TYPE_Q4_K 12u
 #define EDGEXPU_CUDA_TYPE_Q5_K 13u
 #define EDGEXPU_CUDA_TYPE_Q6_K 14u
+/* Paged caches, beside F16 (the GGUF id of bfloat16; no weight of this type is read). */
+#define EDGEXPU_CUDA_TYPE_BF16 30u
 
 int edgexpu_cuda_abi_version(void);
 
@@ -295,6 +298,110 @@ int edgexpu_cuda_llama_forward(void *session, const uint32_t *tokens, int n_toke
                                float top_p, uint64_t *rng, uint32_t *next_token, float *last_hidden, char *error,
                                size_t error_size);
 int edgexpu_cuda_llama_close(void *session);
+
+/* ---- a paged key/value cache that many sequences share ------------------------------------------
+ * No counterpart in the reference, whose cache holds one sequence.  The cache is memory that the
+ * caller holds; every call reads it through this descriptor and none keeps anything of it.
+ *
+ * Position p of sequence s (a row of `table`) lies in page table[s][p / page_size], at slot
+ * p % page_size.  A page may be named by several rows (a common prompt); refs counts them, and a
+ * page with refs 0 is free.  A row's entries past its length are -1.  An empty cache is: table all
+ * -1, lens and refs all 0.  The calls below keep these rules; memory that breaks them gives an error
+ * of the next edgexpu_cuda_stream_sync and no access outside the pools.
+ *
+ * All calls are ordered on `stream` and neither synchronise nor allocate, so they can be captured.
+ * Calls that change the cache use its `work` memory: one at a time, ordered against each other and
+ * against the calls that read the cache, as for any buffer.  Entries of a batch whose sequence is
+ * negative are skipped (the idle slots of a batch of fixed size). */
+typedef struct edgexpu_cuda_kv_cache {
+    void *k, *v;           /* device, 16-byte aligned: [n_layers][n_pages][n_kv][page_size][head_dim] */
+    int64_t layer_stride;  /* elements from a layer to the next, in k and in v; a multiple of 8 */
+    int64_t page_stride;   /* elements from a page to the next; a multiple of 8, >= a page's elements */
+    uint32_t type;         /* EDGEXPU_CUDA_TYPE_F16 or _BF16 */
+    int n_layers;
+    int n_pages;
+    int page_size;         /* 16, 32, 64, 128 or 256 tokens */
+    int n_kv;              /* key/value heads */
+    int head_dim;          /* a multiple of 8, 256 at most */
+    int n_seqs;            /* rows of table, and entries of lens */
+    int max_pages;         /* columns of table */
+    int32_t *table;        /* device [n_seqs][max_pages] */
+    int32_t *lens;         /* device [n_seqs]: tokens held */
+    int32_t *refs;         /* device [n_pages] */
+    int32_t *work;         /* device scratch of the page calls, edgexpu_cuda_kv_work_bytes bytes; NULL for
+                              a cache that is only read and written to */
+} edgexpu_cuda_kv_cache;
+
+/* Bytes of `work` for a cache of n_pages pages and n_seqs rows. */
+size_t edgexpu_cuda_kv_work_bytes(int n_pages, int n_seqs);
+
+/* Room for n_new[i] >= 0 more tokens at the end of sequence seqs[i], i < n (device arrays; n at most
+ * 4096, no sequence twice).  Pages are taken in the order of the batch, lowest free page first.  Where
+ * the last page holds tokens and another row names it too, the sequence gets a page of its own with
+ * those tokens copied, in all layers (of the rows of one batch that share such a page and are all its
+ * holders, the last one keeps it).  pos[i] (device, nullable) receives the position of the first new
+ * token.  All or nothing: without pages for the whole batch nothing changes, pos is -1, and *missing
+ * (device, nullable) is the number of pages that were short, else 0; with missing NULL, a shortage is
+ * an error of the next edgexpu_cuda_stream_sync.  An entry that does not fit its row, or is not a
+ * sequence, is left out (pos -1) and an error of the next sync. */
+int edgexpu_cuda_kv_append_dev(const edgexpu_cuda_kv_cache *cache, const int32_t *seqs, const int32_t *n_new, int n,
+                               int32_t *pos, int32_t *missing, void *stream);
+/* Sequence dst[i], empty, becomes a copy of src[i] that shares its pages; no data moves (append copies
+ * a shared last page when a sharer grows).  No dst twice, and no src among the dst. */
+int edgexpu_cuda_kv_fork_dev(const edgexpu_cuda_kv_cache *cache, const int32_t *src, const int32_t *dst, int n,
+                             void *stream);
+/* Cut sequence seqs[i] to its first keep[i] tokens (keep NULL: to none) and give its other pages back;
+ * a page is free when no row names it any more. */
+int edgexpu_cuda_kv_free_dev(const edgexpu_cuda_kv_cache *cache, const int32_t *seqs, const int32_t *keep, int n,
+                             void *stream);
+/* The data of page src[i] into page dst[i], in all layers (tables and refs stay).  A page is a
+ * destination once at most and not both source and destination, else its data are undefined. */
+int edgexpu_cuda_kv_copy_dev(const edgexpu_cuda_kv_cache *cache, const int32_t *src, const int32_t *dst, int n,
+                             void *stream);
+/* Move the pages in use to the low end of the pool: with L pages in use, the i-th of them at or above L
+ * goes to the i-th free page below L, and tables and refs follow.  *n_live (device, nullable) = L. */
+int edgexpu_cuda_kv_compact_dev(const edgexpu_cuda_kv_cache *cache, int32_t *n_live, void *stream);
+
+/* How the rotation pairs the elements of a head: (2j, 2j + 1), or (j, j + rope_dims / 2). */
+#define EDGEXPU_CUDA_ROPE_ADJACENT 0
+#define EDGEXPU_CUDA_ROPE_HALVES 1
+/* Query, key and value heads of n_tokens new tokens, one pass from the projections' fp32 rows to the
+ * attention's operands: q and k are RMS-normed per head (x / sqrt(mean(x^2) + eps) * weight[head_dim];
+ * a NULL weight: not normed) and rotated by the cos/sin row of their position in `rope`
+ * [rope_positions][rope_dims] (cos, sin of pair 0, of pair 1, ...; NULL: not rotated), then rounded to
+ * the cache's type: q to q_out [n_tokens][n_heads][head_dim], k and v into `layer` of the cache at
+ * position pos[t] of sequence seqs[t].  Rows are q_stride, k_stride and v_stride floats apart
+ * (multiples of 4, pointers 16-byte aligned), so the parts of one q|k|v row serve.  Tokens whose
+ * sequence or position is negative are padding: q_out 0, nothing stored.  A token without a page, or
+ * whose position is past rope_positions, is treated so too and is an error of the next sync. */
+int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache *cache, int layer, const float *q, const float *k,
+                                  const float *v, int64_t q_stride, int64_t k_stride, int64_t v_stride, int n_tokens,
+                                  int n_heads, const float *q_weight, const float *k_weight, float eps,
+                                  const float *rope, int rope_positions, int rope_dims, int rope_pairing,
+                                  const int32_t *seqs, const int32_t *pos, void *q_out, void *stream);
+
+/* Attention of n_tokens queries, the last tokens of n_batch sequences, over `layer` of the cache:
+ *   out[t][h] = sum_j softmax_j(scale * dot(q[t][h], K[j][h / rep])) V[j][h / rep],  rep = n_heads / n_kv,
+ * over the positions j up to t's own.  Entry i's tokens are q_start[i] .. q_start[i + 1] - 1 (device,
+ * n_batch + 1 values from 0 to n_tokens; NULL: one token each, n_tokens = n_batch) and are the last of the
+ * lens[seqs[i]] tokens of its sequence, which the cache already holds.  A token that sees no position, or
+ * whose sequence is negative, gets 0.  Memory past a sequence's end is not used, whatever it holds.
+ *
+ * A shared prefix: the first shared_len positions of every sequence of the batch hold what those of row
+ * shared_seq hold (the same pages, or copies), and are read once for the whole batch.  At most
+ * lens[shared_seq] positions are shared; 0: none.
+ *
+ * q and out are [n_tokens][n_heads][head_dim], 16-byte aligned; q of the cache's type, out of out_type: that type or
+ * EDGEXPU_CUDA_TYPE_F32 (the next linear's input).  Products are of the cache's type (the softmax weights
+ * are rounded to it), sums are fp32.  max_len bounds the sequences' lengths for the division of the work
+ * only.  work: edgexpu_cuda_kv_attention_work_bytes bytes of device memory, 256-byte aligned, of this call's own until it
+ * is done; the size depends on these numbers alone. */
+int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache *cache, int layer, const void *q, const int32_t *seqs,
+                                  const int32_t *q_start, int n_batch, int n_tokens, int n_heads, int shared_seq,
+                                  int shared_len, int max_len, float scale, void *out, uint32_t out_type, void *work,
+                                  size_t work_bytes, void *stream);
+size_t edgexpu_cuda_kv_attention_work_bytes(const edgexpu_cuda_kv_cache *cache, int n_batch, int n_tokens, int n_heads,
+                                            int shared_len, int max_len);
 
 /* Token id encoded in an argmax key (0 when no row had a finite score). */
 static inline uint32_t edgexpu_cuda_argmax_key_id(uint64_t key) {
