@@ -399,25 +399,47 @@ struct QkArgs {
   int rope_positions, rot, halves;
   const int32_t *seqs, *pos;
   uint16_t* q_out;
+  enum { NONE, IN_LANE, BETWEEN_LANES, IN_SHARED } form;  // where a pair is turned
 };
 
 constexpr int QK_WARPS = 8;
+constexpr int QK_HEADS = 4;  // heads a group of lanes holds at once: their loads are all in flight together
 
-// A warp a head of a token: its elements as float4 (lane, lane + 32), the sum of squares in fp32 over
-// the warp, the normed row through shared memory so that either pairing finds its partners, and one
-// 8-byte store per four elements.  Bound by HBM: 4 bytes read and 2 written an element.
-template <typename T>
-__global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvView c, const QkArgs a) {
+// Pair (y0, y1) by the angle (c, s).
+__device__ __forceinline__ void rotate(float& y0, float& y1, float c, float s) {
+  const float a = y0 * c - y1 * s;
+  y1 = y0 * s + y1 * c;
+  y0 = a;
+}
+
+// A group of GS lanes takes QK_HEADS heads of a token, a lane V times four elements of each: the
+// token's page and angles are looked up once for them, the sums of squares are fp32 over the group, and
+// a pair is turned in its lane (adjacent), between two lanes (halves, in whole chunks of four) or, for
+// the other splits of a head, in shared memory.  Bound by HBM (4 bytes read and 2 written an element).
+template <typename T, int GS, int V>
+__global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvView c, const QkArgs a, const int units) {
   pdl_enter_grid();
-  __shared__ __align__(16) float rows[QK_WARPS][256];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int per_token = a.n_heads + 2 * c.n_kv;
-  const long long item = static_cast<long long>(blockIdx.x) * QK_WARPS + w;
-  if (item >= static_cast<long long>(a.n_tokens) * per_token) return;
-  const int t = static_cast<int>(item / per_token), h = static_cast<int>(item % per_token);
-  const int kind = h < a.n_heads ? 0 : h < a.n_heads + c.n_kv ? 1 : 2;  // q, k, v
-  const int hh = kind == 0 ? h : kind == 1 ? h - a.n_heads : h - a.n_heads - c.n_kv;
-  const int s = a.seqs[t], p = a.pos[t], nv = c.hd / 4;
+  constexpr int GROUPS = 32 / GS;
+  extern __shared__ __align__(16) float rows[];  // [warp][group][QK_HEADS][GS * V * 4], for the last form only
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, gl = lane % GS, gr = lane / GS;
+  const long long unit = static_cast<long long>(blockIdx.x) * QK_WARPS + w;
+  const int t = static_cast<int>(unit / units);
+  if (t >= a.n_tokens) return;
+  const int per_token = a.n_heads + 2 * c.n_kv, nv = c.hd / 4;
+  const int h0 = (static_cast<int>(unit % units) * GROUPS + gr) * QK_HEADS;
+  float4 e[QK_HEADS][V];
+#pragma unroll
+  for (int i = 0; i < QK_HEADS; ++i) {
+    const int h = h0 + i;
+    const float* x = h < a.n_heads           ? a.q + t * a.qs + static_cast<long long>(h) * c.hd
+                     : h < a.n_heads + c.n_kv ? a.k + t * a.ks + static_cast<long long>(h - a.n_heads) * c.hd
+                                              : a.v + t * a.vs + static_cast<long long>(h - a.n_heads - c.n_kv) * c.hd;
+#pragma unroll
+    for (int u = 0; u < V; ++u)
+      e[i][u] = h < per_token && gl + u * GS < nv ? __ldcs(reinterpret_cast<const float4*>(x) + gl + u * GS)
+                                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  const int s = a.seqs[t], p = a.pos[t];
   bool live = s >= 0 && p >= 0;
   int page = -1;
   if (live) {
@@ -428,69 +450,142 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvVie
       if (lane == 0) atomicOr(c.status, ST_BAD_CACHE);
     }
   }
-  uint16_t* dst;
-  if (kind == 0) {
-    dst = a.q_out + (static_cast<long long>(t) * a.n_heads + hh) * c.hd;
-  } else {
-    if (!live) return;
-    dst = (kind == 1 ? c.k : c.v) + a.layer * c.layer_stride + page * c.page_stride +
-          ((static_cast<long long>(hh) << c.ps_shift) + (p & ((1 << c.ps_shift) - 1))) * c.hd;
-  }
-  if (!live) {
-    for (int i = lane; i < nv; i += 32) reinterpret_cast<uint2*>(dst)[i] = make_uint2(0u, 0u);
-    return;
-  }
-  const float* x = kind == 0 ? a.q + t * a.qs : kind == 1 ? a.k + t * a.ks : a.v + t * a.vs;
-  const float4* x4 = reinterpret_cast<const float4*>(x + static_cast<long long>(hh) * c.hd);
-  float4 e[2];
-  float ss = 0.0f;
+  const float* cs = a.rope != nullptr && live ? a.rope + static_cast<long long>(p) * a.rot : nullptr;
+  const int half = a.rot / 2;
+
+  // 1 / rms of each head, and the norm's weights
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int j = lane + i * 32;
-    e[i] = j < nv ? x4[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    ss += e[i].x * e[i].x + e[i].y * e[i].y + e[i].z * e[i].z + e[i].w * e[i].w;
-  }
-  if (kind < 2) {
-    const float* wt = kind == 0 ? a.qw : a.kw;
+  for (int i = 0; i < QK_HEADS; ++i) {
+    const int h = h0 + i;
+    const float* wt = h < a.n_heads ? a.qw : h < a.n_heads + c.n_kv ? a.kw : nullptr;
+    float ss = 0.0f;
+#pragma unroll
+    for (int u = 0; u < V; ++u) ss += e[i][u].x * e[i][u].x + e[i][u].y * e[i][u].y + e[i][u].z * e[i][u].z + e[i][u].w * e[i][u].w;
+#pragma unroll
+    for (int o = GS / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
     if (wt != nullptr) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
       const float r = 1.0f / sqrtf(ss / static_cast<float>(c.hd) + a.eps);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = lane + i * 32;
+      for (int u = 0; u < V; ++u) {
+        const int j = gl + u * GS;
         if (j < nv) {
-          e[i].x = e[i].x * r * wt[4 * j];
-          e[i].y = e[i].y * r * wt[4 * j + 1];
-          e[i].z = e[i].z * r * wt[4 * j + 2];
-          e[i].w = e[i].w * r * wt[4 * j + 3];
+          const float4 g = reinterpret_cast<const float4*>(wt)[j];
+          e[i][u].x = e[i][u].x * r * g.x;
+          e[i][u].y = e[i][u].y * r * g.y;
+          e[i][u].z = e[i][u].z * r * g.z;
+          e[i][u].w = e[i][u].w * r * g.w;
         }
       }
     }
-    if (a.rope != nullptr) {
-      float* row = rows[w];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (lane + i * 32 < nv) reinterpret_cast<float4*>(row)[lane + i * 32] = e[i];
-      __syncwarp();
-      const float* cs = a.rope + static_cast<long long>(p) * a.rot;
-      const int half = a.rot / 2;
-      for (int j = lane; j < half; j += 32) {
-        const int i0 = a.halves ? j : 2 * j, i1 = a.halves ? j + half : 2 * j + 1;
-        const float cc = cs[2 * j], sn = cs[2 * j + 1], y0 = row[i0], y1 = row[i1];
-        row[i0] = y0 * cc - y1 * sn;
-        row[i1] = y0 * sn + y1 * cc;
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (lane + i * 32 < nv) e[i] = reinterpret_cast<float4*>(row)[lane + i * 32];
-    }
   }
+
+  const int turned = min(QK_HEADS, a.n_heads + c.n_kv - h0);  // q and k heads of the group, may be none
+  if (a.form == QkArgs::IN_LANE) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + i * 32 < nv)
-      reinterpret_cast<uint2*>(dst)[lane + i * 32] = make_uint2(pack16<T>(e[i].x, e[i].y), pack16<T>(e[i].z, e[i].w));
+    for (int u = 0; u < V; ++u) {
+      const int j = gl + u * GS;
+      if (cs != nullptr && 4 * j < a.rot) {
+        const float2 a0 = *reinterpret_cast<const float2*>(cs + 4 * j);
+        const bool both = 4 * j + 2 < a.rot;
+        const float2 a1 = both ? *reinterpret_cast<const float2*>(cs + 4 * j + 2) : make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < QK_HEADS; ++i)
+          if (i < turned) {
+            rotate(e[i][u].x, e[i][u].y, a0.x, a0.y);
+            if (both) rotate(e[i][u].z, e[i][u].w, a1.x, a1.y);
+          }
+      }
+    }
+  } else if (a.form == QkArgs::BETWEEN_LANES) {
+    // V == 1 and half % 4 == 0: chunk j < half / 4 turns with chunk j + half / 4, half / 4 lanes on
+    const int step = half / 4;
+    const bool low = gl < step, in = gl < 2 * step;
+    float ang[8] = {1.0f, 0.0f, 1.0f, 0.0f, 1.0f, 0.0f, 1.0f, 0.0f};
+    if (cs != nullptr && in) {
+      const float2* at = reinterpret_cast<const float2*>(cs) + 4 * (low ? gl : gl - step);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 x = at[k];
+        ang[2 * k] = x.x;
+        ang[2 * k + 1] = low ? -x.y : x.y;  // y0 c - y1 s below, y1 c + y0 s above
+      }
+    }
+    const int from = gr * GS + (low ? gl + step : in ? gl - step : gl);
+#pragma unroll
+    for (int i = 0; i < QK_HEADS; ++i) {
+      const float4 mine = e[i][0];
+      float4 other;
+      other.x = __shfl_sync(0xFFFFFFFFu, mine.x, from);
+      other.y = __shfl_sync(0xFFFFFFFFu, mine.y, from);
+      other.z = __shfl_sync(0xFFFFFFFFu, mine.z, from);
+      other.w = __shfl_sync(0xFFFFFFFFu, mine.w, from);
+      if (i < turned && in && cs != nullptr) {
+        e[i][0].x = mine.x * ang[0] + other.x * ang[1];
+        e[i][0].y = mine.y * ang[2] + other.y * ang[3];
+        e[i][0].z = mine.z * ang[4] + other.z * ang[5];
+        e[i][0].w = mine.w * ang[6] + other.w * ang[7];
+      }
+    }
+  } else if (a.form == QkArgs::IN_SHARED) {
+    float* row = rows + (w * GROUPS + gr) * QK_HEADS * GS * V * 4;
+#pragma unroll
+    for (int i = 0; i < QK_HEADS; ++i)
+#pragma unroll
+      for (int u = 0; u < V; ++u) reinterpret_cast<float4*>(row + i * GS * V * 4)[gl + u * GS] = e[i][u];
+    __syncwarp();
+    for (int j = gl; j < half && cs != nullptr; j += GS)
+      for (int i = 0; i < turned; ++i) rotate(row[i * GS * V * 4 + j], row[i * GS * V * 4 + j + half], cs[2 * j], cs[2 * j + 1]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < QK_HEADS; ++i)
+#pragma unroll
+      for (int u = 0; u < V; ++u) e[i][u] = reinterpret_cast<float4*>(row + i * GS * V * 4)[gl + u * GS];
+  }
+
+#pragma unroll
+  for (int i = 0; i < QK_HEADS; ++i) {
+    const int h = h0 + i;
+    if (h >= per_token) break;
+    uint16_t* dst = a.q_out + (static_cast<long long>(t) * a.n_heads + h) * c.hd;
+    if (h >= a.n_heads) {
+      if (!live) break;
+      const bool is_k = h < a.n_heads + c.n_kv;
+      const int hh = is_k ? h - a.n_heads : h - a.n_heads - c.n_kv;
+      dst = (is_k ? c.k : c.v) + a.layer * c.layer_stride + page * c.page_stride +
+            ((static_cast<long long>(hh) << c.ps_shift) + (p & ((1 << c.ps_shift) - 1))) * c.hd;
+    }
+#pragma unroll
+    for (int u = 0; u < V; ++u)
+      if (gl + u * GS < nv)
+        reinterpret_cast<uint2*>(dst)[gl + u * GS] =
+            live ? make_uint2(pack16<T>(e[i][u].x, e[i][u].y), pack16<T>(e[i][u].z, e[i][u].w)) : make_uint2(0u, 0u);
+  }
+}
+
+template <typename T, int GS, int V>
+cudaError_t launch_heads_as(const KvView& c, QkArgs a, cudaStream_t st) {
+  const int at_once = QK_HEADS * (32 / GS);
+  const int units = (a.n_heads + 2 * c.n_kv + at_once - 1) / at_once;
+  const long long blocks = (static_cast<long long>(a.n_tokens) * units + QK_WARPS - 1) / QK_WARPS;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  if (a.rope == nullptr)
+    a.form = QkArgs::NONE;
+  else if (!a.halves)
+    a.form = QkArgs::IN_LANE;
+  else
+    a.form = V == 1 && a.rot % 8 == 0 ? QkArgs::BETWEEN_LANES : QkArgs::IN_SHARED;
+  const size_t smem = a.form == QkArgs::IN_SHARED ? static_cast<size_t>(QK_WARPS) * 32 * V * QK_HEADS * 16 : 0;
+  if (smem > 48 * 1024) {
+    static const cudaError_t set =
+        cudaFuncSetAttribute(qk_norm_rope_kernel<T, GS, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, QK_WARPS * 32 * V * QK_HEADS * 16);
+    if (set != cudaSuccess) return set;
+  }
+  return launch_dependent(qk_norm_rope_kernel<T, GS, V>, dim3(static_cast<unsigned>(blocks)), dim3(QK_WARPS * 32), smem, st, c, a, units);
+}
+
+template <typename T>
+cudaError_t launch_heads(const KvView& c, const QkArgs& a, cudaStream_t st) {
+  return c.hd <= 64 ? launch_heads_as<T, 16, 1>(c, a, st) : c.hd <= 128 ? launch_heads_as<T, 32, 1>(c, a, st) : launch_heads_as<T, 32, 2>(c, a, st);
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -623,18 +718,16 @@ int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache* cache, int layer,
                         static_cast<long long>(qn), static_cast<long long>(kn));
   if (rope != nullptr && (rope_positions < 1 || rope_dims < 2 || rope_dims > c.hd || rope_dims % 2 != 0))
     return ex::api_fail(nullptr, 0, "qk_norm_rope: a table of %d positions and %d dims for heads of %d", rope_positions, rope_dims, c.hd);
+  if (!ex::aligned(q_weight, 16) || !ex::aligned(k_weight, 16) || !ex::aligned(rope, 8))
+    return ex::api_fail(nullptr, 0, "qk_norm_rope: the norm weights must be 16-byte aligned, the table 8-byte");
   if (rope_pairing != EDGEXPU_CUDA_ROPE_ADJACENT && rope_pairing != EDGEXPU_CUDA_ROPE_HALVES)
     return ex::api_fail(nullptr, 0, "qk_norm_rope: pairing %d", rope_pairing);
   if (n_tokens == 0) return 1;
-  const long long items = static_cast<long long>(n_tokens) * (n_heads + 2LL * c.n_kv);
-  const long long blocks = (items + ex::QK_WARPS - 1) / ex::QK_WARPS;
-  if (blocks > INT_MAX) return ex::api_fail(nullptr, 0, "qk_norm_rope: %d tokens in one call", n_tokens);
   const ex::QkArgs a{q, k, v, q_stride, k_stride, v_stride, n_tokens, n_heads, layer, q_weight, k_weight, eps, rope,
                      rope_positions, rope_dims, rope_pairing == EDGEXPU_CUDA_ROPE_HALVES, seqs, pos,
-                     static_cast<uint16_t*>(q_out)};
-  auto kern = cache->type == ex::TYPE_F16 ? ex::qk_norm_rope_kernel<__half> : ex::qk_norm_rope_kernel<__nv_bfloat16>;
-  return ex::launched(ex::launch_dependent(kern, dim3(static_cast<unsigned>(blocks)), dim3(ex::QK_WARPS * 32), 0,
-                                           static_cast<cudaStream_t>(stream), c, a),
+                     static_cast<uint16_t*>(q_out), ex::QkArgs::NONE};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return ex::launched(cache->type == ex::TYPE_F16 ? ex::launch_heads<__half>(c, a, st) : ex::launch_heads<__nv_bfloat16>(c, a, st),
                       "qk_norm_rope");
 }
 

@@ -371,7 +371,7 @@ int edgexpu_cuda_kv_compact_dev(const edgexpu_cuda_kv_cache *cache, int32_t *n_l
  * [rope_positions][rope_dims] (cos, sin of pair 0, of pair 1, ...; NULL: not rotated), then rounded to
  * the cache's type: q to q_out [n_tokens][n_heads][head_dim], k and v into `layer` of the cache at
  * position pos[t] of sequence seqs[t].  Rows are q_stride, k_stride and v_stride floats apart
- * (multiples of 4, pointers 16-byte aligned), so the parts of one q|k|v row serve.  Tokens whose
+ * (multiples of 4; pointers and weights 16-byte aligned, the table 8), so the parts of one q|k|v row serve.  Tokens whose
  * sequence or position is negative are padding: q_out 0, nothing stored.  A token without a page, or
  * whose position is past rope_positions, is treated so too and is an error of the next sync. */
 int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache *cache, int layer, const float *q, const float *k,
