@@ -69,13 +69,13 @@ __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t v) {
 }
 
 template <typename T>
-__device__ constexpr uint32_t exponent16();  // the bits of the exponent
+__host__ __device__ constexpr uint32_t exponent16();  // the bits of the exponent
 template <>
-__device__ constexpr uint32_t exponent16<__half>() {
+__host__ __device__ constexpr uint32_t exponent16<__half>() {
   return 0x7C00u;
 }
 template <>
-__device__ constexpr uint32_t exponent16<__nv_bfloat16>() {
+__host__ __device__ constexpr uint32_t exponent16<__nv_bfloat16>() {
   return 0x7F80u;
 }
 

@@ -19,85 +19,10 @@
 
 #include "capi_internal.h"
 #include "kv.cuh"
+#include "kvattn.cuh"
 
 namespace ex {
 namespace {
-
-constexpr int TILE = 64;       // positions a tile, a multiple of 64 from position 0: a page never straddles two
-constexpr int MAX_SLOTS = 64;  // parts of a row in the shared pass, and in its own
-// Softmax weights are kept 2^P_SHIFT times as large, in o and l alike, so that f16 holds the small
-// weights of a long row in full: 2^-26 of the largest and more, where 2^-14 would be its limit.
-constexpr float P_SHIFT = 12.0f;
-
-struct AttnArgs {
-  KvView c;
-  long long layer_off;  // elements
-  const uint16_t* q;
-  const int32_t* seqs;
-  const int32_t* q_start;
-  int n_batch, n_tokens, n_heads, rep;
-  int shared_seq, shared_len;
-  float scale;       // times log2(e)
-  int n_pre, n_own;  // parts of the shared prefix, and of a sequence's own positions
-  float* part_o;     // [n_pre + n_own][token][head][hd]
-  float2* part_ml;   // [n_pre + n_own][token][head]: m, l
-  void* out;
-  int out_f32;
-};
-
-// Positions of the prefix.
-__device__ __forceinline__ int shared_of(const AttnArgs& a) {
-  if (a.shared_len <= 0) return 0;
-  const int held = min(a.c.lens[a.shared_seq], a.c.max_pages << a.c.ps_shift);
-  return max(0, min(a.shared_len, held));
-}
-
-struct Entry {
-  int row;         // of the table; -1: idle
-  int t0, nq;      // its tokens
-  int len;         // positions held
-  int start;       // first position of its own pass
-  bool shares;     // it takes part in the shared pass
-};
-
-__device__ __forceinline__ Entry entry_of(const AttnArgs& a, int i, int shared) {
-  Entry e{-1, i, 1, 0, 0, false};
-  if (a.q_start != nullptr) {
-    e.t0 = a.q_start[i];
-    e.nq = a.q_start[i + 1] - e.t0;
-    if (e.t0 < 0 || e.nq < 0 || e.t0 > a.n_tokens || e.nq > a.n_tokens - e.t0) {
-      atomicOr(a.c.status, ST_BAD_CACHE);
-      e.t0 = e.nq = 0;
-      return e;
-    }
-  }
-  const int s = a.seqs[i];
-  if (s < 0) return e;
-  if (s >= a.c.n_seqs) {
-    atomicOr(a.c.status, ST_BAD_CACHE);
-    return e;
-  }
-  e.row = s;
-  const int held = a.c.lens[s], most = a.c.max_pages << a.c.ps_shift;
-  if (held < 0 || held > most) atomicOr(a.c.status, ST_BAD_CACHE);
-  e.len = max(0, min(held, most));
-  e.shares = shared > 0 && e.len - e.nq + 1 >= shared;
-  e.start = e.shares ? shared : 0;
-  return e;
-}
-
-// Tiles of a part: those of [start, end) cut into at most n parts of `per` tiles.
-struct Cut {
-  int first, tiles, per, used;
-};
-__device__ __forceinline__ Cut cut_of(int start, int end, int n) {
-  Cut c;
-  c.first = start / TILE;
-  c.tiles = end > start ? (end + TILE - 1) / TILE - c.first : 0;
-  c.per = max(1, (c.tiles + n - 1) / n);
-  c.used = (c.tiles + c.per - 1) / c.per;
-  return c;
-}
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
@@ -468,6 +393,14 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
   }
 }
 
+// Parts of the shared pass that a token's head has.
+__device__ __forceinline__ int tc_parts(const AttnArgs& a, int shared, int t, int head) {
+  const TcCut c = tc_cut(a, shared);
+  const int kvh = head / a.rep, r = t * a.rep + head - kvh * a.rep;
+  const long long first = (static_cast<long long>(kvh) * c.row_blocks + r / a.pre_rows) * c.tiles;
+  return static_cast<int>((first + c.tiles - 1) / c.per - first / c.per) + 1;
+}
+
 // Join the parts of each (token, head): a warp a row, lane x has elements 4 x ... and 4 x + 128 ...
 template <typename T>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
@@ -491,7 +424,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
   const bool sees = e.row >= 0 && t >= e.t0 && t < e.t0 + e.nq && e.len - e.nq + (t - e.t0) + 1 > 0;
   int n_pre = 0, n_own = 0;
   if (sees) {
-    if (e.shares) n_pre = cut_of(0, shared, a.n_pre).used;
+    if (e.shares) n_pre = a.pre_rows > 0 ? tc_parts(a, shared, t, static_cast<int>(row - static_cast<long long>(t) * a.n_heads)) : cut_of(0, shared, a.n_pre).used;
     n_own = cut_of(e.start, e.len, a.n_own).used;
   }
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
@@ -538,9 +471,10 @@ struct AttnPlan {
   int pre_wm, own_wm;
   int pre_blocks, own_blocks;
   int n_pre, n_own;
+  int pre_rows, pre_ctas;
 };
 
-AttnPlan plan_of(int n_kv, bool ragged, int n_batch, int n_tokens, int n_heads, int shared_len, int max_len) {
+AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n_heads, int shared_len, int max_len) {
   AttnPlan p{};
   const int sms = api_device_info().sm_count > 0 ? api_device_info().sm_count : 148;
   const int rep = n_heads / n_kv;
@@ -555,7 +489,13 @@ AttnPlan plan_of(int n_kv, bool ragged, int n_batch, int n_tokens, int n_heads, 
   const long long target = 4LL * sms;
   const long long own_n = (target + static_cast<long long>(p.own_blocks) * n_kv - 1) / (static_cast<long long>(p.own_blocks) * n_kv);
   p.n_own = static_cast<int>(std::max(1LL, std::min({own_n, static_cast<long long>((own_tiles + 1) / 2), static_cast<long long>(MAX_SLOTS)})));
-  if (shared_len > 0) {
+  if (shared_len > 0 && (hd == 64 || hd == 128) && rows > 16) {
+    const int tiles = (shared_len + TC_TILE - 1) / TC_TILE;
+    p.pre_rows = rows > 128 ? 256 : 128;
+    const long long blocks = (rows + p.pre_rows - 1) / p.pre_rows * n_kv;
+    p.pre_ctas = static_cast<int>(std::min(static_cast<long long>(sms), blocks * tiles));
+    p.n_pre = static_cast<int>(std::min(static_cast<long long>(tiles), p.pre_ctas / blocks + 2));
+  } else if (shared_len > 0) {
     p.pre_wm = rows <= 16 ? 1 : 4;
     p.pre_blocks = static_cast<int>((rows + 16 * p.pre_wm - 1) / (16 * p.pre_wm));
     const int tiles = (shared_len + TILE - 1) / TILE;
@@ -592,8 +532,11 @@ cudaError_t launch_rows(const AttnArgs& a, int wm, int blocks, int splits, int p
 }
 
 template <typename T>
-cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-  if (p.n_pre > 0) {
+cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, uint32_t type, cudaStream_t st) {
+  if (p.pre_rows > 0) {
+    const cudaError_t e = launch_attn_tc(a, type, st);
+    if (e != cudaSuccess) return e;
+  } else if (p.n_pre > 0) {
     const cudaError_t e = launch_rows<T>(a, p.pre_wm, p.pre_blocks, p.n_pre, 1, st);
     if (e != cudaSuccess) return e;
   }
@@ -614,8 +557,8 @@ size_t edgexpu_cuda_kv_attention_work_bytes(const edgexpu_cuda_kv_cache* cache, 
       max_len < 1 || cache->head_dim < 1)
     return 0;
   // one token each may come with q_start or without: the larger of the two divisions
-  const ex::AttnPlan p = ex::plan_of(cache->n_kv, true, n_batch, n_tokens, n_heads, shared_len, max_len);
-  const ex::AttnPlan u = ex::plan_of(cache->n_kv, false, n_batch, n_tokens, n_heads, shared_len, max_len);
+  const ex::AttnPlan p = ex::plan_of(cache->n_kv, cache->head_dim, true, n_batch, n_tokens, n_heads, shared_len, max_len);
+  const ex::AttnPlan u = ex::plan_of(cache->n_kv, cache->head_dim, false, n_batch, n_tokens, n_heads, shared_len, max_len);
   return std::max(ex::work_bytes(p, n_tokens, n_heads, cache->head_dim), ex::work_bytes(u, n_tokens, n_heads, cache->head_dim));
 }
 
@@ -640,7 +583,7 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   if (max_len < 1) return ex::api_fail(nullptr, 0, "kv_attention: max_len %d", max_len);
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return ex::api_fail(nullptr, 0, "kv_attention: q and out must be 16-byte aligned");
-  const ex::AttnPlan p = ex::plan_of(a.c.n_kv, q_start != nullptr, n_batch, n_tokens, n_heads, shared_len, max_len);
+  const ex::AttnPlan p = ex::plan_of(a.c.n_kv, a.c.hd, q_start != nullptr, n_batch, n_tokens, n_heads, shared_len, max_len);
   const size_t need = ex::work_bytes(p, n_tokens, n_heads, a.c.hd);
   const long long rows = static_cast<long long>(n_tokens) * n_heads;
   if (rows > INT_MAX || p.own_blocks < 1) return ex::api_fail(nullptr, 0, "kv_attention: %d tokens in one call", n_tokens);
@@ -660,14 +603,16 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   a.scale = scale * 1.4426950408889634f;
   a.n_pre = p.n_pre;
   a.n_own = p.n_own;
+  a.pre_rows = p.pre_rows;
+  a.pre_ctas = p.pre_ctas;
   const int slots = p.n_pre + p.n_own;
   a.part_ml = static_cast<float2*>(work);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + (static_cast<size_t>(slots) * rows * 8 + 15) / 16 * 16);
   a.out = out;
   a.out_f32 = out_type == ex::TYPE_F32;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = cache->type == ex::TYPE_F16 ? ex::launch_attention_as<__half>(a, p, st)
-                                                    : ex::launch_attention_as<__nv_bfloat16>(a, p, st);
+  const cudaError_t e = cache->type == ex::TYPE_F16 ? ex::launch_attention_as<__half>(a, p, cache->type, st)
+                                                    : ex::launch_attention_as<__nv_bfloat16>(a, p, cache->type, st);
   if (e != cudaSuccess) return ex::api_fail(nullptr, 0, "kv_attention: %s", cudaGetErrorString(e));
   return 1;
 }

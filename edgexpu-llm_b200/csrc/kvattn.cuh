@@ -1,0 +1,106 @@
+// kvattn.cuh -- what the kernels of attention over a paged cache share (kvattn.cu, kvattn_tc.cu).
+#pragma once
+
+#include "kv.cuh"
+
+namespace ex {
+
+constexpr int TILE = 64;       // positions a tile, a multiple of 64 from position 0: a page never straddles two
+constexpr int MAX_SLOTS = 64;  // parts of a row in the shared pass, and in its own
+// Softmax weights are kept 2^P_SHIFT times as large, in o and l alike, so that f16 holds the small
+// weights of a long row in full: 2^-24 of the largest and more, where 2^-14 would be its limit.
+constexpr float P_SHIFT = 10.0f;
+
+struct AttnArgs {
+  KvView c;
+  long long layer_off;  // elements
+  const uint16_t* q;
+  const int32_t* seqs;
+  const int32_t* q_start;
+  int n_batch, n_tokens, n_heads, rep;
+  int shared_seq, shared_len;
+  float scale;       // times log2(e)
+  int n_pre, n_own;  // parts of the shared prefix, and of a sequence's own positions
+  int pre_rows;      // rows a block of the tensor-memory kernel's shared pass; 0: the rows kernel makes it
+  int pre_ctas;      // its blocks
+  float* part_o;     // [n_pre + n_own][token][head][hd]
+  float2* part_ml;   // [n_pre + n_own][token][head]: m, l
+  void* out;
+  int out_f32;
+};
+
+// Positions of the prefix.
+__device__ __forceinline__ int shared_of(const AttnArgs& a) {
+  if (a.shared_len <= 0) return 0;
+  const int held = min(a.c.lens[a.shared_seq], a.c.max_pages << a.c.ps_shift);
+  return max(0, min(a.shared_len, held));
+}
+
+struct Entry {
+  int row;         // of the table; -1: idle
+  int t0, nq;      // its tokens
+  int len;         // positions held
+  int start;       // first position of its own pass
+  bool shares;     // it takes part in the shared pass
+};
+
+__device__ __forceinline__ Entry entry_of(const AttnArgs& a, int i, int shared) {
+  Entry e{-1, i, 1, 0, 0, false};
+  if (a.q_start != nullptr) {
+    e.t0 = a.q_start[i];
+    e.nq = a.q_start[i + 1] - e.t0;
+    if (e.t0 < 0 || e.nq < 0 || e.t0 > a.n_tokens || e.nq > a.n_tokens - e.t0) {
+      atomicOr(a.c.status, ST_BAD_CACHE);
+      e.t0 = e.nq = 0;
+      return e;
+    }
+  }
+  const int s = a.seqs[i];
+  if (s < 0) return e;
+  if (s >= a.c.n_seqs) {
+    atomicOr(a.c.status, ST_BAD_CACHE);
+    return e;
+  }
+  e.row = s;
+  const int held = a.c.lens[s], most = a.c.max_pages << a.c.ps_shift;
+  if (held < 0 || held > most) atomicOr(a.c.status, ST_BAD_CACHE);
+  e.len = max(0, min(held, most));
+  e.shares = shared > 0 && e.len - e.nq + 1 >= shared;
+  e.start = e.shares ? shared : 0;
+  return e;
+}
+
+// Tiles of a part: those of [start, end) cut into at most n parts of `per` tiles.
+struct Cut {  // of the rows kernel
+  int first, tiles, per, used;
+};
+__device__ __forceinline__ Cut cut_of(int start, int end, int n) {
+  Cut c;
+  c.first = start / TILE;
+  c.tiles = end > start ? (end + TILE - 1) / TILE - c.first : 0;
+  c.per = max(1, (c.tiles + n - 1) / n);
+  c.used = (c.tiles + c.per - 1) / c.per;
+  return c;
+}
+
+// The shared pass of the tensor-memory kernel.  Its blocks of rows (kv head outside, rows inside) times
+// the prefix's tiles are one line of work, cut into pre_ctas equal pieces; a block of rows is then
+// divided over the pieces that touch it, and piece c's part of it is slot c - (the first such piece).
+constexpr int TC_TILE = 128;  // positions
+struct TcCut {
+  int tiles, row_blocks;
+  long long total, per;
+};
+__device__ __forceinline__ TcCut tc_cut(const AttnArgs& a, int shared) {
+  TcCut c;
+  c.tiles = (shared + TC_TILE - 1) / TC_TILE;
+  c.row_blocks = (a.n_tokens * a.rep + a.pre_rows - 1) / a.pre_rows;
+  c.total = static_cast<long long>(c.row_blocks) * a.c.n_kv * c.tiles;
+  c.per = (c.total + a.pre_ctas - 1) / a.pre_ctas;
+  return c;
+}
+
+// Launch the shared pass on the tensor cores' own memory (kvattn_tc.cu); hd is 64 or 128.
+cudaError_t launch_attn_tc(const AttnArgs& a, uint32_t type, cudaStream_t st);
+
+}  // namespace ex
