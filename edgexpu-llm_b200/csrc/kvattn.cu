@@ -20,6 +20,7 @@
 #include "capi_internal.h"
 #include "kv.cuh"
 #include "kvattn.cuh"
+#include "kvattn_mma.cuh"
 
 namespace ex {
 namespace {
@@ -32,47 +33,6 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two neighbouring outputs of a row whose sums are o and weight l.  A row that sees nothing is 0; one
-// that sees only scores of -inf is 0/0, as its softmax is.
-template <typename T>
-__device__ __forceinline__ void store_out(const AttnArgs& a, long long at, float o0, float o1, float l, bool sees) {
-  const float r = 1.0f / l;
-  o0 = sees ? o0 * r : 0.0f;
-  o1 = sees ? o1 * r : 0.0f;
-  if (a.out_f32)
-    *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(o0, o1);
-  else
-    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) = pack16<T>(o0, o1);
 }
 
 template <int DP, int WM>
@@ -401,14 +361,15 @@ __device__ __forceinline__ int tc_parts(const AttnArgs& a, int shared, int t, in
   return static_cast<int>((first + c.tiles - 1) / c.per - first / c.per) + 1;
 }
 
-// Join the parts of each (token, head): a warp a row, lane x has elements 4 x ... and 4 x + 128 ...
+// Join the parts of each (token, head): a warp a row, lane x has elements 4 x ... and 4 x + 128 ...  The
+// parts' weights come first, a lane a part, then their sums eight at a time.
 template <typename T>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
   pdl_enter_grid();
   const int lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= static_cast<long long>(a.n_tokens) * a.n_heads) return;
-  const int t = static_cast<int>(row / a.n_heads), hd = a.c.hd;
+  const int t = static_cast<int>(row / a.n_heads), head = static_cast<int>(row - static_cast<long long>(t) * a.n_heads), hd = a.c.hd;
   int i = t;
   if (a.q_start != nullptr) {  // the last entry that starts at or before t
     int lo = 0, up = a.n_batch;
@@ -423,37 +384,70 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
   const Entry e = entry_of(a, i, shared);
   const bool sees = e.row >= 0 && t >= e.t0 && t < e.t0 + e.nq && e.len - e.nq + (t - e.t0) + 1 > 0;
   int n_pre = 0, n_own = 0;
+  long long cont = 0;  // single tokens: the row of the second own part
   if (sees) {
-    if (e.shares) n_pre = a.pre_rows > 0 ? tc_parts(a, shared, t, static_cast<int>(row - static_cast<long long>(t) * a.n_heads)) : cut_of(0, shared, a.n_pre).used;
-    n_own = cut_of(e.start, e.len, a.n_own).used;
+    if (e.shares) n_pre = a.pre_rows > 0 ? tc_parts(a, shared, t, head) : cut_of(0, shared, a.n_pre).used;
+    if (a.own_ctas > 0) {
+      const int tiles = cut_of(e.start, e.len, 1).tiles;
+      if (tiles > 0) {
+        const int kvh = head / a.rep, r = head - kvh * a.rep, n_rb = (a.rep + 15) / 16, per_entry = a.c.n_kv * n_rb;
+        const long long per = (static_cast<long long>(a.own_off[a.n_batch]) * per_entry + a.own_ctas - 1) / a.own_ctas;
+        const long long first = static_cast<long long>(a.own_off[i]) * per_entry + static_cast<long long>(kvh * n_rb + r / 16) * tiles;
+        const int c0 = static_cast<int>(first / per);
+        n_own = static_cast<int>((first + tiles - 1) / per) - c0 + 1;
+        cont = a.cont_row0 + static_cast<long long>(c0 + 1) * 16 + r % 16;
+      }
+    } else {
+      n_own = cut_of(e.start, e.len, a.n_own).used;
+    }
   }
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
   const int n = n_pre + n_own;
-  // part x < n: slots 0 .. n_pre - 1, then a.n_pre ...
-  auto slot_of = [&](int x) { return static_cast<long long>(x < n_pre ? x : a.n_pre + x - n_pre) * rows + row; };
-  float top = -INFINITY;
-  for (int x = lane; x < n; x += 32) top = fmaxf(top, a.part_ml[slot_of(x)].x);
+  auto row_of = [&](int x) {
+    if (x < n_pre) return x * rows + row;
+    x -= n_pre;
+    return a.own_ctas > 0 && x > 0 ? cont + 16LL * (x - 1) : (a.n_pre + x) * rows + row;
+  };
+  float top = -INFINITY, l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int b = 0; b < n; b += 32) {
+    const float2 ml = b + lane < n ? a.part_ml[row_of(b + lane)] : make_float2(-INFINITY, 0.0f);
+    float most = ml.x;
 #pragma unroll
-  for (int y = 16; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, y));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int x = 0; x < n; ++x) {
-    const float2 ml = a.part_ml[slot_of(x)];
-    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing seen: its sums are not written
-    const float f = exp2f(ml.x - base);
-    l += f * ml.y;
-    const float* src = a.part_o + slot_of(x) * hd;
+    for (int y = 16; y > 0; y >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, y));
+    const float before = top;
+    top = fmaxf(top, most);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float f = exp2f(ml.x - base), g = exp2f(before - base);
+    float lw = f * ml.y;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int d = lane * 4 + k * 128;
-      if (d < hd) {
-        const float4 v = *reinterpret_cast<const float4*>(src + d);
-        o[4 * k] += f * v.x;
-        o[4 * k + 1] += f * v.y;
-        o[4 * k + 2] += f * v.z;
-        o[4 * k + 3] += f * v.w;
+    for (int y = 16; y > 0; y >>= 1) lw += __shfl_xor_sync(0xFFFFFFFFu, lw, y);
+    l = l * g + lw;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] *= g;
+    const bool none = ml.x == -INFINITY && ml.y == 0.0f;  // nothing seen: its sums may not be written
+    for (int x0 = 0; x0 < min(32, n - b); x0 += 8) {
+      float4 v[8][2];
+      float w[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        w[x] = __shfl_sync(0xFFFFFFFFu, f, x0 + x);
+        const bool skip = __shfl_sync(0xFFFFFFFFu, static_cast<int>(none), x0 + x) != 0;
+        const float* src = a.part_o + row_of(b + x0 + x) * hd;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int d = lane * 4 + k * 128;
+          v[x][k] = !skip && d < hd ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
       }
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          o[4 * k] += w[x] * v[x][k].x;
+          o[4 * k + 1] += w[x] * v[x][k].y;
+          o[4 * k + 2] += w[x] * v[x][k].z;
+          o[4 * k + 3] += w[x] * v[x][k].w;
+        }
     }
   }
 #pragma unroll
@@ -472,6 +466,8 @@ struct AttnPlan {
   int pre_blocks, own_blocks;
   int n_pre, n_own;
   int pre_rows, pre_ctas;
+  bool one;      // single tokens: kvattn_one.cu
+  int own_ctas;
 };
 
 AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n_heads, int shared_len, int max_len) {
@@ -479,17 +475,29 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
   const int sms = api_device_info().sm_count > 0 ? api_device_info().sm_count : 148;
   const int rep = n_heads / n_kv;
   const long long rows = static_cast<long long>(n_tokens) * rep;
-  p.own_wm = rows <= 16LL * n_batch ? 1 : 4;
-  const int own_rows = 16 * p.own_wm;
-  p.own_blocks = static_cast<int>(ragged ? (rows + own_rows - 1) / own_rows + n_batch
-                                         : static_cast<long long>(n_batch) * ((rep + own_rows - 1) / own_rows));
   shared_len = std::max(0, std::min(shared_len, max_len));
   const int own_tiles = (std::max(0, max_len - shared_len) + TILE - 1) / TILE + 1;
-  // two blocks an SM: enough parts for two rounds of them, none shorter than two tiles
-  const long long target = 4LL * sms;
-  const long long own_n = (target + static_cast<long long>(p.own_blocks) * n_kv - 1) / (static_cast<long long>(p.own_blocks) * n_kv);
-  p.n_own = static_cast<int>(std::max(1LL, std::min({own_n, static_cast<long long>((own_tiles + 1) / 2), static_cast<long long>(MAX_SLOTS)})));
-  if (shared_len > 0 && (hd == 64 || hd == 128) && rows > 16) {
+  p.one = !ragged && hd <= 128 && n_batch <= ONE_MAX_BATCH;
+  p.n_own = 1;
+  if (p.one) {
+    // short runs and no prefix: a block each, which needs no join; a tile takes a block about 0.5 us, a join 3
+    const long long runs = static_cast<long long>(n_batch) * n_kv * ((rep + 15) / 16);
+    if ((shared_len > 0 || own_tiles > 8) && runs * own_tiles <= INT_MAX)
+      p.own_ctas = static_cast<int>(std::min(static_cast<long long>(attn_one_blocks(hd, rep, n_batch)), runs * own_tiles));
+    else if (shared_len > 0)
+      p.one = false;
+  }
+  if (!p.one) {
+    p.own_wm = rows <= 16LL * n_batch ? 1 : 4;
+    const int own_rows = 16 * p.own_wm;
+    p.own_blocks = static_cast<int>(ragged ? (rows + own_rows - 1) / own_rows + n_batch
+                                           : static_cast<long long>(n_batch) * ((rep + own_rows - 1) / own_rows));
+    // two blocks an SM: enough parts for two rounds of them, none shorter than two tiles
+    const long long target = 4LL * sms, at_once = static_cast<long long>(p.own_blocks) * n_kv;
+    p.n_own = static_cast<int>(std::max(1LL, std::min({(target + at_once - 1) / at_once, static_cast<long long>((own_tiles + 1) / 2),
+                                                      static_cast<long long>(MAX_SLOTS)})));
+  }
+  if (shared_len > 0 && hd <= 128 && rows > 16) {
     const int tiles = (shared_len + TC_TILE - 1) / TC_TILE;
     p.pre_rows = rows > 128 ? 256 : 128;
     const long long blocks = (rows + p.pre_rows - 1) / p.pre_rows * n_kv;
@@ -505,10 +513,18 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
   return p;
 }
 
-size_t work_bytes(const AttnPlan& p, int n_tokens, int n_heads, int hd) {
+// Rows of partial sums: a slot of every (token, head) for each part, and 16 for each block of the single tokens' line.
+long long part_rows(const AttnPlan& p, int n_tokens, int n_heads) {
   const int slots = p.n_pre + p.n_own;
-  if (slots <= 1) return 256;
-  return static_cast<size_t>(slots) * n_tokens * n_heads * (static_cast<size_t>(hd) * 4 + 8) + 256;
+  if (slots == 1 && p.own_ctas == 0) return 0;
+  return static_cast<long long>(slots) * n_tokens * n_heads + 16LL * p.own_ctas;
+}
+
+size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+size_t work_bytes(const AttnPlan& p, int n_batch, int n_tokens, int n_heads, int hd) {
+  const size_t rows = static_cast<size_t>(part_rows(p, n_tokens, n_heads));
+  return up256(rows * 8) + up256(rows * hd * 4) + up256((static_cast<size_t>(n_batch) + 1) * 4);
 }
 
 template <typename T, int DP, int WM>
@@ -540,8 +556,8 @@ cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, uint32_t t
     const cudaError_t e = launch_rows<T>(a, p.pre_wm, p.pre_blocks, p.n_pre, 1, st);
     if (e != cudaSuccess) return e;
   }
-  const cudaError_t e = launch_rows<T>(a, p.own_wm, p.own_blocks, p.n_own, 0, st);
-  if (e != cudaSuccess || p.n_pre + p.n_own == 1) return e;
+  const cudaError_t e = p.one ? launch_attn_one(a, type, st) : launch_rows<T>(a, p.own_wm, p.own_blocks, p.n_own, 0, st);
+  if (e != cudaSuccess || part_rows(p, a.n_tokens, a.n_heads) == 0) return e;
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
   return launch_dependent(attn_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, st, a);
 }
@@ -559,7 +575,7 @@ size_t edgexpu_cuda_kv_attention_work_bytes(const edgexpu_cuda_kv_cache* cache, 
   // one token each may come with q_start or without: the larger of the two divisions
   const ex::AttnPlan p = ex::plan_of(cache->n_kv, cache->head_dim, true, n_batch, n_tokens, n_heads, shared_len, max_len);
   const ex::AttnPlan u = ex::plan_of(cache->n_kv, cache->head_dim, false, n_batch, n_tokens, n_heads, shared_len, max_len);
-  return std::max(ex::work_bytes(p, n_tokens, n_heads, cache->head_dim), ex::work_bytes(u, n_tokens, n_heads, cache->head_dim));
+  return std::max(ex::work_bytes(p, n_batch, n_tokens, n_heads, cache->head_dim), ex::work_bytes(u, n_batch, n_tokens, n_heads, cache->head_dim));
 }
 
 int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer, const void* q, const int32_t* seqs,
@@ -584,9 +600,9 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return ex::api_fail(nullptr, 0, "kv_attention: q and out must be 16-byte aligned");
   const ex::AttnPlan p = ex::plan_of(a.c.n_kv, a.c.hd, q_start != nullptr, n_batch, n_tokens, n_heads, shared_len, max_len);
-  const size_t need = ex::work_bytes(p, n_tokens, n_heads, a.c.hd);
+  const size_t need = ex::work_bytes(p, n_batch, n_tokens, n_heads, a.c.hd);
   const long long rows = static_cast<long long>(n_tokens) * n_heads;
-  if (rows > INT_MAX || p.own_blocks < 1) return ex::api_fail(nullptr, 0, "kv_attention: %d tokens in one call", n_tokens);
+  if (rows > INT_MAX || p.own_blocks < 0) return ex::api_fail(nullptr, 0, "kv_attention: %d tokens in one call", n_tokens);
   if (work == nullptr || work_size < need || (reinterpret_cast<uintptr_t>(work) & 255) != 0)
     return ex::api_fail(nullptr, 0, "kv_attention: work memory of %zu bytes, 256-byte aligned, is needed (got %zu)", need,
                         work == nullptr ? static_cast<size_t>(0) : work_size);
@@ -605,9 +621,13 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   a.n_own = p.n_own;
   a.pre_rows = p.pre_rows;
   a.pre_ctas = p.pre_ctas;
-  const int slots = p.n_pre + p.n_own;
-  a.part_ml = static_cast<float2*>(work);
-  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + (static_cast<size_t>(slots) * rows * 8 + 15) / 16 * 16);
+  a.own_ctas = p.own_ctas;
+  const size_t parts = static_cast<size_t>(ex::part_rows(p, n_tokens, n_heads));
+  uint8_t* at = static_cast<uint8_t*>(work);
+  a.part_ml = reinterpret_cast<float2*>(at);
+  a.part_o = reinterpret_cast<float*>(at + ex::up256(parts * 8));
+  a.own_off = reinterpret_cast<int*>(at + ex::up256(parts * 8) + ex::up256(parts * a.c.hd * 4));
+  a.cont_row0 = static_cast<long long>(p.n_pre + p.n_own) * rows;
   a.out = out;
   a.out_f32 = out_type == ex::TYPE_F32;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1,5 +1,8 @@
-// kvattn.cuh -- what the kernels of attention over a paged cache share (kvattn.cu, kvattn_tc.cu).
+// kvattn.cuh -- what the kernels of attention over a paged cache share (kvattn.cu, kvattn_one.cu,
+// kvattn_tc.cu).
 #pragma once
+
+#include <cuda.h>
 
 #include "kv.cuh"
 
@@ -10,6 +13,7 @@ constexpr int MAX_SLOTS = 64;  // parts of a row in the shared pass, and in its 
 // Softmax weights are kept 2^P_SHIFT times as large, in o and l alike, so that f16 holds the small
 // weights of a long row in full: 2^-24 of the largest and more, where 2^-14 would be its limit.
 constexpr float P_SHIFT = 10.0f;
+constexpr float GROW = 5.0f;  // a reference maximum moves when the maximum is this much larger: weights stay below 2^15
 
 struct AttnArgs {
   KvView c;
@@ -23,6 +27,9 @@ struct AttnArgs {
   int n_pre, n_own;  // parts of the shared prefix, and of a sequence's own positions
   int pre_rows;      // rows a block of the tensor-memory kernel's shared pass; 0: the rows kernel makes it
   int pre_ctas;      // its blocks
+  int own_ctas;      // blocks of the single-token kernel, whose line of work is cut into equal pieces; 0: a run each
+  int* own_off;      // [n_batch + 1]: tiles of the line before each entry's run (by the kernel, for the join)
+  long long cont_row0;  // row of part_o, part_ml where the blocks' 16 continuing rows begin
   float* part_o;     // [n_pre + n_own][token][head][hd]
   float2* part_ml;   // [n_pre + n_own][token][head]: m, l
   void* out;
@@ -100,7 +107,30 @@ __device__ __forceinline__ TcCut tc_cut(const AttnArgs& a, int shared) {
   return c;
 }
 
-// Launch the shared pass on the tensor cores' own memory (kvattn_tc.cu); hd is 64 or 128.
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A layer of a pool as [page][head x slot][element], in boxes of 64 elements of at most `most` of a
+// page's positions; elements past head_dim read as 0 (kvattn_tc.cu).
+bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type, int most);
+
+// Launch the single tokens' own pass (kvattn_one.cu), hd at most 128; its blocks where the line is cut.
+constexpr int ONE_MAX_BATCH = 2048;  // the runs' offsets are in shared memory
+cudaError_t launch_attn_one(const AttnArgs& a, uint32_t type, cudaStream_t st);
+int attn_one_blocks(int hd, int rep, int n_batch);
+
+// Launch the shared pass on the tensor cores' own memory (kvattn_tc.cu), hd at most 128.
 cudaError_t launch_attn_tc(const AttnArgs& a, uint32_t type, cudaStream_t st);
 
 }  // namespace ex

@@ -27,7 +27,6 @@ namespace ex {
 namespace {
 
 constexpr int TC_THREADS = 384;
-constexpr float GROW = 5.0f;  // with P_SHIFT = 10, weights stay below 2^15, inside f16
 
 template <int DP, int MT>
 struct TcLayout {
@@ -94,20 +93,6 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t leading) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -328,7 +313,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int half = (warp - 4) >> 2, r = threadIdx.x & 127;  // the thread's row of its half
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_at = lane_base + 128 * half, o_at = lane_base + 256 + 128 * half;
-    const int rows = a.n_tokens * a.rep;
+    const int rows = a.n_tokens * a.rep, hd = a.c.hd;
     const float sc = fabsf(a.scale);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale: -Q, so that a maximum is a maximum
     uint32_t segs = 0, tiles_done = 0;
@@ -342,9 +327,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int x = r; x < 128 * CH; x += 128) {
         const int qr = x / CH, ch = x % CH, rr = base_row + qr;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (rr < rows) {
+        if (rr < rows && ch * 8 < hd) {
           const int tok = rr / a.rep, head = g.kvh * a.rep + rr - tok * a.rep;
-          v = *reinterpret_cast<const uint4*>(a.q + (static_cast<long long>(tok) * a.n_heads + head) * DP + ch * 8);
+          v = *reinterpret_cast<const uint4*>(a.q + (static_cast<long long>(tok) * a.n_heads + head) * hd + ch * 8);
           v.x ^= flip;
           v.y ^= flip;
           v.z ^= flip;
@@ -437,10 +422,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tc_ld32(o_at + c, o);
         tc_wait_ld();
         if (rr < rows) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + part * DP + c);
+          float4* dst = reinterpret_cast<float4*>(a.part_o + part * hd + c);
 #pragma unroll
           for (int x = 0; x < 8; ++x)
-            dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]),
+            if (c + 4 * x < hd) dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]),
                                  __uint_as_float(o[4 * x + 3]));
         }
       }
@@ -479,19 +464,22 @@ EncodeTiledFn kv_encode_tiled() {
   return fn;
 }
 
-// A layer of a pool as [page][head x slot][element], in boxes of 64 elements of a page's positions.
-bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type) {
+}  // namespace
+
+bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type, int most) {
   EncodeTiledFn enc = kv_encode_tiled();
   if (enc == nullptr) return false;
   const int ps = 1 << c.ps_shift;
   const cuuint64_t dims[3] = {(cuuint64_t)c.hd, (cuuint64_t)c.n_kv * ps, (cuuint64_t)c.n_pages};
   const cuuint64_t strides[2] = {(cuuint64_t)c.hd * 2, (cuuint64_t)c.page_stride * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)(ps < TC_TILE ? ps : TC_TILE), 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(ps < most ? ps : most), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   return enc(map, type == TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
              const_cast<uint16_t*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+namespace {
 
 template <typename T, int DP, int MT>
 cudaError_t launch_tc_as(const AttnArgs& a, uint32_t type, cudaStream_t st) {
@@ -499,13 +487,13 @@ cudaError_t launch_tc_as(const AttnArgs& a, uint32_t type, cudaStream_t st) {
   static const cudaError_t set = cudaFuncSetAttribute(attn_tc_kernel<T, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
   if (set != cudaSuccess) return set;
   CUtensorMap kmap, vmap;
-  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type)) return cudaErrorInvalidValue;
+  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type, TC_TILE) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type, TC_TILE)) return cudaErrorInvalidValue;
   return launch_dependent(attn_tc_kernel<T, DP, MT>, dim3(a.pre_ctas), dim3(TC_THREADS), L::ALLOC, st, a, kmap, vmap);
 }
 
 template <typename T>
 cudaError_t launch_tc(const AttnArgs& a, uint32_t type, cudaStream_t st) {
-  if (a.c.hd == 64) return a.pre_rows == 128 ? launch_tc_as<T, 64, 1>(a, type, st) : launch_tc_as<T, 64, 2>(a, type, st);
+  if (a.c.hd <= 64) return a.pre_rows == 128 ? launch_tc_as<T, 64, 1>(a, type, st) : launch_tc_as<T, 64, 2>(a, type, st);
   return a.pre_rows == 128 ? launch_tc_as<T, 128, 1>(a, type, st) : launch_tc_as<T, 128, 2>(a, type, st);
 }
 
