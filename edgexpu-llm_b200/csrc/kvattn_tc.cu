@@ -27,6 +27,9 @@ namespace ex {
 namespace {
 
 constexpr int TC_THREADS = 384;
+#ifndef POLY_OF_8
+#define POLY_OF_8 0
+#endif
 
 template <int DP, int MT>
 struct TcLayout {
@@ -35,7 +38,7 @@ struct TcLayout {
   static constexpr int SLOTS = (208 * 1024 - MT * SLOT) / SLOT < 10 ? (208 * 1024 - MT * SLOT) / SLOT : 10;
   static constexpr int RING = MT * SLOT;
   static constexpr int BARS = RING + SLOTS * SLOT;
-  static constexpr int N_BARS = 2 * SLOTS + 4 * 2 + 1;
+  static constexpr int N_BARS = 2 * SLOTS + 8 * 2 + 1;
   static constexpr int MISC = BARS + 8 * N_BARS;
   static constexpr int ALLOC = MISC + 16 + 1024;
   static_assert(ALLOC > 116 * 1024 && ALLOC <= 227 * 1024, "one block an SM, which then owns the tensor memory");
@@ -50,21 +53,32 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// One product of the tensor pipe, D = A B or D += A B.  Descriptors come as their low words (the address
+// and the leading offset); the high word is one constant.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<int>(add))
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<int>(add)), "n"(DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<int>(add))
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<int>(add)), "n"(DESC_HI)
       : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 #define EX_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
@@ -90,9 +104,57 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
 // Rows of 128 bytes with the 128-byte swizzle, groups of eight 1024 bytes apart.  Read along the 64
 // elements of a row (Q, K) the leading offset is not used; read across the rows (V) it is the distance
 // to the next 64 elements.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t leading) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+__device__ __forceinline__ uint32_t sw128_desc(uint32_t addr, uint32_t leading) {  // the low word
+  return (addr >> 4) | (leading >> 4) << 16;
+}
+
+// Pairs of fp32 in one instruction.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 two(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 one_by_one(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The larger; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of a pair without the special-function units, for x <= 16: x = n + f with n the nearest integer
+// (found in the low bits of x + 1.5 2^23), 2^f by the minimax polynomial of degree 4 on [-1/2, 1/2] with
+// value 1 at 0 (Remez exchange; relative error 3.6e-6, below the weights' rounding to 11 bits), and n
+// added to the exponent.  At and below -127 the result is 0.  A NaN is not kept.
+__device__ __forceinline__ float2 exp2_poly(f32x2 x) {
+  constexpr float MAGIC = 12582912.0f;
+  const float2 c = one_by_one(x);
+  x = two(fmaxf(c.x, -127.0f), fmaxf(c.y, -127.0f));
+  const f32x2 t = add2(x, two(MAGIC, MAGIC));
+  const f32x2 f = add2(x, fma2(t, two(-1.0f, -1.0f), two(MAGIC, MAGIC)));
+  f32x2 p = two(0.009782912f, 0.009782912f);
+  p = fma2(p, f, two(0.055976883f, 0.055976883f));
+  p = fma2(p, f, two(0.24020711f, 0.24020711f));
+  p = fma2(p, f, two(0.69311362f, 0.69311362f));
+  p = fma2(p, f, two(1.0f, 1.0f));
+  const float2 n = one_by_one(t), v = one_by_one(p);
+  return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(n.x) << 23)),
+                     __int_as_float(__float_as_int(v.y) + (__float_as_int(n.y) << 23)));
 }
 
 __device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -118,13 +180,21 @@ struct Ring {
       phase ^= 1u;
     }
   }
+  __device__ __forceinline__ void back() {
+    if (--slot < 0) {
+      slot = NS - 1;
+      phase ^= 1u;
+    }
+  }
 };
 
-// A block of rows along consecutive tiles of the prefix.
+// A block of rows along consecutive tiles of the prefix, in steps of half a tile.
+constexpr int STEP = TC_TILE / 2;
 struct Segment {
   int kvh, row0, tile0, n, slot;
+  int steps;  // the prefix's last half tile may be empty
 };
-__device__ __forceinline__ Segment segment_at(const TcCut& c, long long at, long long end, int pre_rows) {
+__device__ __forceinline__ Segment segment_at(const TcCut& c, long long at, long long end, int pre_rows, int shared) {
   Segment s;
   const long long block = at / c.tiles;
   s.tile0 = static_cast<int>(at - block * c.tiles);
@@ -132,6 +202,7 @@ __device__ __forceinline__ Segment segment_at(const TcCut& c, long long at, long
   s.kvh = static_cast<int>(block / c.row_blocks);
   s.row0 = static_cast<int>(block - static_cast<long long>(s.kvh) * c.row_blocks) * pre_rows;
   s.slot = static_cast<int>(blockIdx.x - block * c.tiles / c.per);
+  s.steps = min(2 * s.n, (shared - s.tile0 * TC_TILE + STEP - 1) / STEP);
   return s;
 }
 
@@ -140,22 +211,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using L = TcLayout<DP, MT>;
   constexpr int CH = DP / 8, NS = L::SLOTS;
+  constexpr bool FINE = MT == 1;  // P in two numbers of the type, a coarse and the rest
   constexpr uint32_t FMT = exponent16<T>() == exponent16<__half>() ? 0u : 1u;
-  // D fp32, A and B of the type, M = 128; N = 128 for S, DP for O, whose B is read across its rows
-  constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  // D fp32, A and B of the type, M = 128; N = 64 for S, DP for O, whose B is read across its rows
+  constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t(STEP) >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t IDESC_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t(DP) >> 3) << 17) | ((128u >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);  // a ring slot's boxes landed
   uint64_t* empty = full + NS;                                   // the products that read it are done
   uint64_t* q_full = empty + NS;                                 // [half]: Q is in shared memory (128 threads)
-  uint64_t* s_full = q_full + 2;                                 // [half]: S is in tensor memory
-  uint64_t* p_full = s_full + 2;                                 // [half]: P is (128 threads)
-  uint64_t* o_full = p_full + 2;                                 // [half]: the segment's O is
-  uint64_t* fin = o_full + 2;
+  uint64_t* q_free = q_full + 2;                                 // [half]: the segment's sums have left Q's memory (4 warps)
+  uint64_t* s_full = q_free + 2;                                 // [half][buffer]: S is in tensor memory
+  uint64_t* p_full = s_full + 4;                                 // [half][buffer]: P is (4 warps)
+  uint64_t* o_done = p_full + 4;                                 // [half][buffer]: the P V of a step is in O
+  uint64_t* fin = o_done + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -164,9 +237,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 128);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&q_free[i], 4);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&s_full[2 * i + j], 1);
+        mbar_init(&p_full[2 * i + j], 4);
+        mbar_init(&o_done[2 * i + j], 1);
+      }
     }
     mbar_init(fin, 1);
     *abort_flag = 0;
@@ -180,16 +256,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
   pdl_enter_grid();
 
-  const int shared = shared_of(a);
+  const int shared = __shfl_sync(0xFFFFFFFFu, shared_of(a), 0);
   const TcCut cut = tc_cut(a, shared);
   const long long begin = blockIdx.x * cut.per, end = min(cut.total, begin + cut.per);
 
-  // registers: 384 x 168 at launch, from here on 128 x 64 and 256 x 216 (a row's 128 scores and 32 of O)
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // K of tile 0, V of tile 0, K of tile 1, ...: the order in which the products need them
     const int box = min(1 << a.c.ps_shift, TC_TILE);  // positions a box holds
@@ -198,7 +271,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     int issued = 0;  // slots filled, NS at most
     bool ok = true;
     for (long long at = begin; ok && at < end;) {
-      const Segment g = segment_at(cut, at, end, a.pre_rows);
+      const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
       for (int i = 0; ok && i < g.n; ++i) {
         const int p0 = (g.tile0 + i) * TC_TILE;
@@ -242,64 +315,92 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if (!drained) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t q_s = smem_u32(smem), ring_s = smem_u32(smem + L::RING);
-      Ring<NS> ring;
-      uint32_t segs = 0, tiles_done = 0;
-      bool ok = true;
-      auto slot_ready = [&](const Ring<NS>& r) { return spin(&full[r.slot], r.phase, abort_flag); };
-      auto product_s = [&](int half, int slot) {
-        const uint64_t qd = sw128_desc(q_s + half * L::SLOT, 16), kd = sw128_desc(ring_s + slot * L::SLOT, 16);
+    // The warp runs the loop together and one thread issues: descriptors are then uniform where they are made.
+    const uint32_t q_s = smem_u32(smem), ring_s = smem_u32(smem + L::RING);
+    const bool lead = elect_one();
+    Ring<NS> ring;
+    uint32_t segs = 0, used[2] = {0, 0};  // P of either buffer taken so far, in each half
+    bool ok = true;
+    auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, spin(bar, parity, abort_flag)) != 0; };
+    // S of 64 positions, the first or last of a tile, into the buffer of that parity
+    auto product_s = [&](int half, int slot, int b) {
+      const uint32_t qd = sw128_desc(q_s + half * L::SLOT, 16), kd = sw128_desc(ring_s + slot * L::SLOT + b * (STEP * 128), 16);
+      if (lead) {
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-          const uint64_t off = static_cast<uint64_t>(((k / 4) * L::HALF + (k % 4) * 32) >> 4);
-          mma_ss(tmem + 128 * half, qd + off, kd + off, IDESC_S, k > 0);
+          const uint32_t off = ((k / 4) * L::HALF + (k % 4) * 32) >> 4;
+          mma_ss(tmem + 128 * half + STEP * b, qd + off, kd + off, IDESC_S, k > 0);
         }
-        tc_commit(&s_full[half]);
-      };
-      for (long long at = begin; ok && at < end; ++segs) {
-        const Segment g = segment_at(cut, at, end, a.pre_rows);
-        at += g.n;
-        ok = slot_ready(ring);
+        tc_commit(&s_full[2 * half + b]);
+      }
+      __syncwarp();
+    };
+    auto give_back = [&](int slot) {
+      if (lead) tc_commit(&empty[slot]);
+      __syncwarp();
+    };
+    for (long long at = begin; ok && at < end; ++segs) {
+      const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
+      at += g.n;
+      Ring<NS> k = ring, v = ring;  // K and V of the tiles in use; V comes after K
+      v.next();
+      ok = there(&full[k.slot], k.phase);
+#pragma unroll
+      for (int h = 0; h < MT; ++h) {
+        ok = ok && there(&q_full[h], segs & 1u);
+        if (!ok) break;
+        tc_after();
+        product_s(h, k.slot, 0);
+      }
+      if (!ok) break;
+      if (g.steps > 1)
+#pragma unroll
+        for (int h = 0; h < MT; ++h) product_s(h, k.slot, 1);
+      give_back(k.slot);
+      for (int j = 0; j < g.steps; ++j) {
+        const int b = j & 1;
+        if (b == 0) ok = there(&full[v.slot], v.phase);
+        if (b == 0 && j + 2 < g.steps) {  // the next tile's K, two places on
+          k.next();
+          k.next();
+        }
 #pragma unroll
         for (int h = 0; h < MT; ++h) {
-          ok = ok && spin(&q_full[h], segs & 1u, abort_flag);
+          ok = ok && there(&p_full[2 * h + b], used[b] & 1u);
           if (!ok) break;
           tc_after();
-          product_s(h, ring.slot);
+          const uint32_t vd = sw128_desc(ring_s + v.slot * L::SLOT + b * (STEP * 128), L::HALF);
+          const uint32_t p_at = tmem + 128 * h + STEP * b;
+          if (lead) {
+#pragma unroll
+            for (int s = 0; s < STEP / 16; ++s) {
+              const uint32_t vs = vd + ((s * 2048) >> 4);
+              mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, j > 0 || s > 0);
+              if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
+            }
+            tc_commit(&o_done[2 * h + b]);
+          }
+          __syncwarp();
+          if (j + 2 < g.steps) {
+            if (b == 0 && h == 0) ok = there(&full[k.slot], k.phase);
+            if (!ok) break;
+            product_s(h, k.slot, b);
+          }
         }
         if (!ok) break;
-        tc_commit(&empty[ring.slot]);
-        ring.next();
-        for (int i = 0; i < g.n; ++i, ++tiles_done) {
-          const bool more = i + 1 < g.n;
-          const Ring<NS> v = ring;
-          ring.next();
-          const Ring<NS> k = ring;
-          if (more) ring.next();
-          ok = slot_ready(v);
-#pragma unroll
-          for (int h = 0; h < MT; ++h) {
-            ok = ok && spin(&p_full[h], tiles_done & 1u, abort_flag);
-            if (!ok) break;
-            tc_after();
-            const uint64_t vd = sw128_desc(ring_s + v.slot * L::SLOT, L::HALF);
-#pragma unroll
-            for (int s = 0; s < TC_TILE / 16; ++s)
-              mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 8 * s, vd + static_cast<uint64_t>((s * 2048) >> 4), IDESC_O, i > 0 || s > 0);
-            if (more) {
-              if (h == 0) ok = slot_ready(k);
-              if (!ok) break;
-              product_s(h, k.slot);
-            } else {
-              tc_commit(&o_full[h]);
-            }
-          }
-          if (!ok) break;
-          tc_commit(&empty[v.slot]);
-          if (more) tc_commit(&empty[k.slot]);
+        ++used[b];
+        if (j + 2 < g.steps && (b == 1 || j + 3 == g.steps)) give_back(k.slot);
+        if (b == 1 || j + 1 == g.steps) {
+          give_back(v.slot);
+          v.next();
+          v.next();
         }
       }
+      // v has moved past this segment's last V, to the place after the next segment's first K
+      ring = v;
+      ring.back();
+    }
+    if (lead) {
       if (!ok) {
         *abort_flag = 1;
         atomicOr(a.c.status, ST_TIMEOUT_FULL);
@@ -307,64 +408,102 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       tc_commit(fin);  // all products are done before tensor memory is given back
       if (!mbar_wait(fin, 0)) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
     }
-  }
-  } else if (warp < 4 + 4 * MT) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    __syncwarp();
+  } else if (warp >= 4 && warp < 4 + 4 * MT) {
     const int half = (warp - 4) >> 2, r = threadIdx.x & 127;  // the thread's row of its half
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_at = lane_base + 128 * half, o_at = lane_base + 256 + 128 * half;
+    const uint32_t o_at = lane_base + 256 + 128 * half;
     const int rows = a.n_tokens * a.rep, hd = a.c.hd;
     const float sc = fabsf(a.scale);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale: -Q, so that a maximum is a maximum
-    uint32_t segs = 0, tiles_done = 0;
-    Ring<NS> ring;
+    uint32_t segs = 0, used[2] = {0, 0};  // S of either buffer so far
+    Ring<NS> ring;  // V of the tile in use
+    ring.next();
     bool ok = true;
     for (long long at = begin; ok && at < end; ++segs) {
-      const Segment g = segment_at(cut, at, end, a.pre_rows);
+      const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
       const int base_row = g.row0 + half * 128;
-#pragma unroll 4
-      for (int x = r; x < 128 * CH; x += 128) {
-        const int qr = x / CH, ch = x % CH, rr = base_row + qr;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (rr < rows && ch * 8 < hd) {
-          const int tok = rr / a.rep, head = g.kvh * a.rep + rr - tok * a.rep;
-          v = *reinterpret_cast<const uint4*>(a.q + (static_cast<long long>(tok) * a.n_heads + head) * hd + ch * 8);
-          v.x ^= flip;
-          v.y ^= flip;
-          v.z ^= flip;
-          v.w ^= flip;
+      {  // a thread takes one chunk of eight elements of every (128 / CH)th row
+        constexpr int STEP = 128 / CH;
+        const int ch = r % CH, dq = STEP / a.rep, dr = STEP - dq * a.rep;
+        int tok = (base_row + r / CH) / a.rep, gh = base_row + r / CH - tok * a.rep;
+        uint4 v[CH];
+#pragma unroll
+        for (int x = 0; x < CH; ++x) {
+          v[x] = tok < a.n_tokens && ch * 8 < hd ? *reinterpret_cast<const uint4*>(
+                                                       a.q + (static_cast<long long>(tok) * a.n_heads + g.kvh * a.rep + gh) * hd + ch * 8)
+                                                 : make_uint4(0u, 0u, 0u, 0u);
+          tok += dq;
+          gh += dr;
+          if (gh >= a.rep) {
+            gh -= a.rep;
+            ++tok;
+          }
         }
-        *reinterpret_cast<uint4*>(smem + half * L::SLOT + (ch / 8) * L::HALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v;
+        if (segs > 0) ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&q_free[half], (segs - 1u) & 1u, abort_flag));
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < CH; ++x) {
+          const int qr = r / CH + x * STEP;
+          v[x].x ^= flip;
+          v[x].y ^= flip;
+          v[x].z ^= flip;
+          v[x].w ^= flip;
+          *reinterpret_cast<uint4*>(smem + half * L::SLOT + (ch / 8) * L::HALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v[x];
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&q_full[half]);
 
       float m = -INFINITY, l = 0.0f;
-      for (int i = 0; i < g.n; ++i, ++tiles_done) {
-        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&s_full[half], tiles_done & 1u, abort_flag));
+      for (int j = 0; j < g.steps; ++j) {
+        const int b = j & 1;
+        const uint32_t s_at = lane_base + 128 * half + STEP * b;
+        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&s_full[2 * half + b], used[b] & 1u, abort_flag));
         if (!ok) break;
+        ++used[b];
         tc_after();
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) tc_ld32(s_at + c, s + c);
+        uint32_t s[STEP];
+        tc_ld32(s_at, s);
+        tc_ld32(s_at + 32, s + 32);
         tc_wait_ld();
-        const int valid = shared - (g.tile0 + i) * TC_TILE;
-        if (valid < TC_TILE) {
+        const int valid = shared - g.tile0 * TC_TILE - j * STEP;
+        if (valid < STEP) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
+          for (int c = 0; c < STEP; ++c)
             if (c >= valid) s[c] = 0xFF800000u;
-        }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (half == 0) {
+            // V past the prefix's end is what memory held: 0 for the product
+            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
+            if (!ok) break;
+            uint8_t* vs = smem + L::RING + ring.slot * L::SLOT + b * (STEP * 128);
+            for (int x = valid * 8 + r; x < STEP * 8; x += 128)
 #pragma unroll
-        for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(s[c]));
-        const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
-        if (i == 0) {
+              for (int h = 0; h < DP / 64; ++h) *reinterpret_cast<uint4*>(vs + h * L::HALF + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+        }
+        if (b == 1) {  // on to the next tile's V
+          ring.next();
+          ring.next();
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top[c] = __uint_as_float(s[c]);
+#pragma unroll
+        for (int c = 4; c < STEP; ++c) top[c & 3] = max_nan(top[c & 3], __uint_as_float(s[c]));
+        const float tm = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * sc;
+        if (j == 0) {
           m = tm;
         } else {
-          const bool grow = tm > m + GROW || (m == -INFINITY && tm > m);
+          const bool grow = !(tm <= m + GROW);  // a NaN too
           if (__any_sync(0xFFFFFFFFu, grow)) {
-            // the products before this S are done, and none is running on O
+            // once the last step's product is in O, none runs on it until this step's P is there (the one
+            // before the last was in O before this S, so that the barrier's parity says which)
+            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&o_done[2 * half + (b ^ 1)], (used[b ^ 1] - 1u) & 1u, abort_flag));
+            if (!ok) break;
+            tc_after();
             const float f = grow ? exp2f(m - tm) : 1.0f;
             l *= f;
             if (grow) m = tm;
@@ -379,35 +518,43 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
           }
         }
-        const float base = (m == -INFINITY ? 0.0f : m) - P_SHIFT;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // scores of +inf make the row NaN (inf - inf), as a NaN does; a row of -inf so far has weights 0
+        const float base = m == INFINITY ? NAN : (m == -INFINITY ? 0.0f : m) - P_SHIFT;
+        const f32x2 scale2 = two(sc, sc), base2 = two(-base, -base);
+        f32x2 sum[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
+        uint32_t rest[FINE ? STEP / 2 : 1];
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(s[c]), sc, -base)), p1 = ex2(fmaf(__uint_as_float(s[c + 1]), sc, -base));
-          sum[(c >> 1) & 1] += p0;
-          sum[2 + ((c >> 1) & 1)] += p1;
-          s[c >> 1] = pack16<T>(p0, p1);
+        for (int c = 0; c < STEP; c += 2) {
+          const f32x2 x = fma2(two(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, base2);
+          float2 p;
+          if ((c / 2) % 8 < POLY_OF_8) {
+            p = exp2_poly(x);
+          } else {
+            const float2 y = one_by_one(x);
+            p = make_float2(ex2(y.x), ex2(y.y));
+          }
+          sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], two(p.x, p.y));
+          s[c >> 1] = pack16<T>(p.x, p.y);
+          if constexpr (FINE) {
+            const float2 h = unpack16<T>(s[c >> 1]);
+            rest[c >> 1] = pack16<T>(p.x - h.x, p.y - h.y);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tc_st32(s_at, s);
-        tc_st32(s_at + 32, s + 32);
-        ring.next();  // past K
-        if (valid < TC_TILE && half == 0) {
-          // V past the prefix's end is what memory held: 0 for the product
-          ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
-          if (!ok) break;
-          uint8_t* vs = smem + L::RING + ring.slot * L::SLOT;
-          for (int x = valid * 8 + r; x < TC_TILE * 8; x += 128)
-#pragma unroll
-            for (int h = 0; h < DP / 64; ++h) *reinterpret_cast<uint4*>(vs + h * L::HALF + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        ring.next();  // past V
+        if constexpr (FINE) tc_st32(s_at + STEP / 2, rest);
+        const float2 l01 = one_by_one(add2(sum[0], sum[1]));
+        l += l01.x + l01.y;
         tc_wait_st();
         tc_before();
-        mbar_arrive(&p_full[half]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * half + b]);
       }
-      ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&o_full[half], segs & 1u, abort_flag));
+      if (g.steps & 1) {
+        ring.next();
+        ring.next();
+      }
+      const int last = (g.steps - 1) & 1;
+      ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&o_done[2 * half + last], (used[last] - 1u) & 1u, abort_flag));
       if (!ok) break;
       tc_after();
       const int rr = base_row + r;
@@ -415,22 +562,31 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const long long row = static_cast<long long>(tok) * a.n_heads + g.kvh * a.rep + min(rr, rows - 1) - tok * a.rep;
       const long long part = static_cast<long long>(g.slot) * a.n_tokens * a.n_heads + row;
       if (rr < rows) a.part_ml[part] = make_float2(m, l);
+      // a warp's 32 rows, 32 columns at a time, through Q's memory (its products are done), so that the
+      // stores are whole rows; chunks of a row are swapped by the row
+      uint8_t* mine = smem + half * L::SLOT + (warp & 3) * (L::SLOT / 4);
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
         __syncwarp();
         tc_ld32(o_at + c, o);
         tc_wait_ld();
-        if (rr < rows) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + part * hd + c);
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            if (c + 4 * x < hd) dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]),
-                                 __uint_as_float(o[4 * x + 3]));
+        for (int x = 0; x < 8; ++x)
+          *reinterpret_cast<uint4*>(mine + lane * 128 + ((x ^ (lane & 7)) << 4)) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {  // four rows of 32 columns
+          const int q = 4 * y + (lane >> 3), ch = lane & 7;
+          const long long to = __shfl_sync(0xFFFFFFFFu, part, q);
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + q * 128 + ((ch ^ (q & 7)) << 4));
+          if (base_row + (warp & 3) * 32 + q < rows && c + 4 * ch < hd)
+            *reinterpret_cast<uint4*>(a.part_o + to * hd + c + 4 * ch) = v;
         }
       }
-      __syncwarp();
       tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_free[half]);
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
