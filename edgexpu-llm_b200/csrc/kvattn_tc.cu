@@ -318,87 +318,78 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     // The warp runs the loop together and one thread issues: descriptors are then uniform where they are made.
     const uint32_t q_s = smem_u32(smem), ring_s = smem_u32(smem + L::RING);
     const bool lead = elect_one();
-    Ring<NS> ring;
-    uint32_t segs = 0, used[2] = {0, 0};  // P of either buffer taken so far, in each half
+    Ring<NS> v;  // V of the tile in use; K of the next one is the place after it
+    v.next();
+    uint32_t segs = 0, par[2] = {0, 0};  // parity of either buffer's next P; constant indices only
     bool ok = true;
     auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, spin(bar, parity, abort_flag)) != 0; };
     // S of 64 positions, the first or last of a tile, into the buffer of that parity
-    auto product_s = [&](int half, int slot, int b) {
-      const uint32_t qd = sw128_desc(q_s + half * L::SLOT, 16), kd = sw128_desc(ring_s + slot * L::SLOT + b * (STEP * 128), 16);
-      if (lead) {
+    auto product_s = [&](int half, uint32_t kd, int b) {
+      const uint32_t qd = sw128_desc(q_s + half * L::SLOT, 16);
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t off = ((k / 4) * L::HALF + (k % 4) * 32) >> 4;
-          mma_ss(tmem + 128 * half + STEP * b, qd + off, kd + off, IDESC_S, k > 0);
-        }
-        tc_commit(&s_full[2 * half + b]);
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t off = ((k / 4) * L::HALF + (k % 4) * 32) >> 4;
+        mma_ss(tmem + 128 * half + STEP * b, qd + off, kd + off + ((b * STEP * 128) >> 4), IDESC_S, k > 0);
       }
-      __syncwarp();
-    };
-    auto give_back = [&](int slot) {
-      if (lead) tc_commit(&empty[slot]);
-      __syncwarp();
+      tc_commit(&s_full[2 * half + b]);
     };
     for (long long at = begin; ok && at < end; ++segs) {
       const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
-      Ring<NS> k = ring, v = ring;  // K and V of the tiles in use; V comes after K
-      v.next();
+      Ring<NS> k = v;
+      k.back();
       ok = there(&full[k.slot], k.phase);
 #pragma unroll
-      for (int h = 0; h < MT; ++h) {
-        ok = ok && there(&q_full[h], segs & 1u);
-        if (!ok) break;
-        tc_after();
-        product_s(h, k.slot, 0);
-      }
+      for (int h = 0; h < MT; ++h) ok = ok && there(&q_full[h], segs & 1u);
       if (!ok) break;
-      if (g.steps > 1)
+      tc_after();
+      if (lead) {
+        const uint32_t kd = sw128_desc(ring_s + k.slot * L::SLOT, 16);
 #pragma unroll
-        for (int h = 0; h < MT; ++h) product_s(h, k.slot, 1);
-      give_back(k.slot);
-      for (int j = 0; j < g.steps; ++j) {
-        const int b = j & 1;
-        if (b == 0) ok = there(&full[v.slot], v.phase);
-        if (b == 0 && j + 2 < g.steps) {  // the next tile's K, two places on
-          k.next();
-          k.next();
-        }
+        for (int h = 0; h < MT; ++h) product_s(h, kd, 0);
+        if (g.steps > 1)
 #pragma unroll
-        for (int h = 0; h < MT; ++h) {
-          ok = ok && there(&p_full[2 * h + b], used[b] & 1u);
-          if (!ok) break;
-          tc_after();
-          const uint32_t vd = sw128_desc(ring_s + v.slot * L::SLOT + b * (STEP * 128), L::HALF);
-          const uint32_t p_at = tmem + 128 * h + STEP * b;
-          if (lead) {
-#pragma unroll
-            for (int s = 0; s < STEP / 16; ++s) {
-              const uint32_t vs = vd + ((s * 2048) >> 4);
-              mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, j > 0 || s > 0);
-              if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
-            }
-            tc_commit(&o_done[2 * h + b]);
-          }
-          __syncwarp();
-          if (j + 2 < g.steps) {
-            if (b == 0 && h == 0) ok = there(&full[k.slot], k.phase);
-            if (!ok) break;
-            product_s(h, k.slot, b);
-          }
-        }
-        if (!ok) break;
-        ++used[b];
-        if (j + 2 < g.steps && (b == 1 || j + 3 == g.steps)) give_back(k.slot);
-        if (b == 1 || j + 1 == g.steps) {
-          give_back(v.slot);
-          v.next();
-          v.next();
-        }
+          for (int h = 0; h < MT; ++h) product_s(h, kd, 1);
+        tc_commit(&empty[k.slot]);
       }
-      // v has moved past this segment's last V, to the place after the next segment's first K
-      ring = v;
-      ring.back();
+      __syncwarp();
+      for (int j = 0; ok && j < g.steps; j += 2) {
+        k.next();
+        k.next();
+        ok = there(&full[v.slot], v.phase) && (j + 2 >= g.steps || there(&full[k.slot], k.phase));
+        const uint32_t kd = sw128_desc(ring_s + k.slot * L::SLOT, 16), vd0 = sw128_desc(ring_s + v.slot * L::SLOT, L::HALF);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (j + b >= g.steps) break;
+          const bool more = j + b + 2 < g.steps;
+#pragma unroll
+          for (int h = 0; h < MT; ++h) {
+            ok = ok && there(&p_full[2 * h + b], par[b]);
+            if (!ok) break;
+            tc_after();
+            if (lead) {
+              const uint32_t p_at = tmem + 128 * h + STEP * b;
+#pragma unroll
+              for (int s = 0; s < STEP / 16; ++s) {
+                const uint32_t vs = vd0 + ((b * STEP * 128 + s * 2048) >> 4);
+                mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, b > 0 || s > 0 || j > 0);
+                if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
+              }
+              tc_commit(&o_done[2 * h + b]);
+              if (more) product_s(h, kd, b);
+            }
+            __syncwarp();
+          }
+          par[b] ^= 1u;
+        }
+        if (lead) {  // both tiles' places are free once these products are done
+          tc_commit(&empty[v.slot]);
+          if (j + 2 < g.steps) tc_commit(&empty[k.slot]);
+        }
+        __syncwarp();
+        v.next();
+        v.next();
+      }
     }
     if (lead) {
       if (!ok) {
@@ -416,7 +407,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int rows = a.n_tokens * a.rep, hd = a.c.hd;
     const float sc = fabsf(a.scale);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale: -Q, so that a maximum is a maximum
-    uint32_t segs = 0, used[2] = {0, 0};  // S of either buffer so far
+    uint32_t segs = 0, par[2] = {0, 0};  // parity of either buffer's next S; constant indices only
     Ring<NS> ring;  // V of the tile in use
     ring.next();
     bool ok = true;
@@ -457,12 +448,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       mbar_arrive(&q_full[half]);
 
       float m = -INFINITY, l = 0.0f;
-      for (int j = 0; j < g.steps; ++j) {
-        const int b = j & 1;
+      auto step = [&](const int j, const int b) {
         const uint32_t s_at = lane_base + 128 * half + STEP * b;
-        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&s_full[2 * half + b], used[b] & 1u, abort_flag));
-        if (!ok) break;
-        ++used[b];
+        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&s_full[2 * half + b], par[b], abort_flag)) != 0;
+        if (!ok) return;
+        par[b] ^= 1u;
         tc_after();
         uint32_t s[STEP];
         tc_ld32(s_at, s);
@@ -475,18 +465,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             if (c >= valid) s[c] = 0xFF800000u;
           if (half == 0) {
             // V past the prefix's end is what memory held: 0 for the product
-            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
-            if (!ok) break;
+            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag)) != 0;
+            if (!ok) return;
             uint8_t* vs = smem + L::RING + ring.slot * L::SLOT + b * (STEP * 128);
             for (int x = valid * 8 + r; x < STEP * 8; x += 128)
 #pragma unroll
               for (int h = 0; h < DP / 64; ++h) *reinterpret_cast<uint4*>(vs + h * L::HALF + x * 16) = make_uint4(0u, 0u, 0u, 0u);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
-        }
-        if (b == 1) {  // on to the next tile's V
-          ring.next();
-          ring.next();
         }
         float top[4];
 #pragma unroll
@@ -501,8 +487,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           if (__any_sync(0xFFFFFFFFu, grow)) {
             // once the last step's product is in O, none runs on it until this step's P is there (the one
             // before the last was in O before this S, so that the barrier's parity says which)
-            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&o_done[2 * half + (b ^ 1)], (used[b ^ 1] - 1u) & 1u, abort_flag));
-            if (!ok) break;
+            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&o_done[2 * half + (b ^ 1)], par[b ^ 1] ^ 1u, abort_flag)) != 0;
+            if (!ok) return;
             tc_after();
             const float f = grow ? exp2f(m - tm) : 1.0f;
             l *= f;
@@ -548,13 +534,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * half + b]);
-      }
-      if (g.steps & 1) {
+      };
+      for (int j = 0; ok && j < g.steps; j += 2) {
+        step(j, 0);
+        if (ok && j + 1 < g.steps) step(j + 1, 1);
         ring.next();
         ring.next();
       }
-      const int last = (g.steps - 1) & 1;
-      ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&o_done[2 * half + last], (used[last] - 1u) & 1u, abort_flag));
+      ok = ok && __all_sync(0xFFFFFFFFu, (g.steps & 1) != 0 ? wait_or_abort(&o_done[2 * half], par[0] ^ 1u, abort_flag)
+                                                            : wait_or_abort(&o_done[2 * half + 1], par[1] ^ 1u, abort_flag));
       if (!ok) break;
       tc_after();
       const int rr = base_row + r;
