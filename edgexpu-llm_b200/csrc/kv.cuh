@@ -90,6 +90,17 @@ __device__ __forceinline__ bool finite16(const uint4& v) {
   return ok;
 }
 
+// Two weights >= 0 as a coarse number of the type each and the rest, both above 0 where the weight is (a
+// product of either with an infinity then has its sign): the coarse one is rounded from a little less
+// than the weight.  Together they hold it to 2^-16 (bf16) or 2^-20 (f16).
+template <typename T>
+__device__ __forceinline__ void split16(float p0, float p1, uint32_t& coarse, uint32_t& rest) {
+  constexpr float LESS = exponent16<T>() == 0x7C00u ? 1.0f - 1.0f / 1024 : 1.0f - 1.0f / 256;
+  coarse = pack16<T>(p0 * LESS, p1 * LESS);
+  const float2 c = unpack16<T>(coarse);
+  rest = pack16<T>(p0 - c.x, p1 - c.y);
+}
+
 // Let the next grid of the stream launch, and wait until the one before has completed.
 __device__ __forceinline__ void pdl_enter_grid() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -25,41 +25,49 @@
 namespace ex {
 namespace {
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+constexpr int ROWS_THREADS = 160;
 
 template <int DP, int WM>
 struct RowsLayout {
   static constexpr int ROWS = 16 * WM;
-  static constexpr int STAGES = DP == 64 ? 4 : DP == 128 ? 3 : 2;
-  static constexpr int Q_BYTES = ROWS * DP * 2;
-  static constexpr int KV_BYTES = TILE * DP * 2;
-  static constexpr int JOIN_BYTES = WM == 1 ? 4 * 16 * DP * 4 : 0;  // over the stages, when they are done with
-  static constexpr int ALLOC = Q_BYTES + STAGES * 2 * KV_BYTES;
-  static_assert(JOIN_BYTES <= STAGES * 2 * KV_BYTES, "the join fits the stages");
+  static constexpr int STAGES = DP == 64 ? 3 : 2;
+  static constexpr int HALF = TILE * 128;
+  static constexpr int KV = HALF * (DP / 64);  // a tile of K, or of V
+  static constexpr int Q_AT = STAGES * 2 * KV;
+  static constexpr int BARS = Q_AT + ROWS * DP * 2;
+  static constexpr int JOIN_BYTES = WM == 1 ? 4 * 16 * DP * 4 : 0;  // over the ring, when it is done with
+  static constexpr int ALLOC = BARS + 16 * STAGES + 64 + 1024;
+  static_assert(JOIN_BYTES <= STAGES * 2 * KV, "the join fits the ring");
 };
 
 // One block: 16 * WM rows of one key/value head against one part of the prefix (PRE) or of an entry's
-// own positions.  Four warps; with WM = 4 each has 16 rows and all positions of a tile, with WM = 1
-// (a single token's heads) all have the same 16 rows and 16 positions of each tile, and join at the
-// end.  Tiles come by 16-byte asynchronous copies into STAGES buffers, chunks of a row swapped by
-// row % 8 so that ldmatrix reads all banks.  P is rounded to the cache's type for its product, as the
-// tensor cores take it; its sum l is of the unrounded values.
+// own positions.  Warp 4 brings K and V by TMA (128-byte swizzle; dims past head_dim read as 0).  Of the
+// other four, with WM = 4 each has 16 rows and all positions of a tile, with WM = 1 all have the same 16
+// rows and 16 positions of each tile, and join at the end.  P is rounded to the cache's type for its
+// product, as the tensor cores take it (with WM = 1, where bytes bound, in two numbers of the type); its
+// sum l is of the unrounded values.
 template <typename T, int DP, int WM>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const int pre) {
+__global__ void __launch_bounds__(ROWS_THREADS)
+    attn_rows_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const int pre) {
   using L = RowsLayout<DP, WM>;
   constexpr int ROWS = L::ROWS, NT = WM == 1 ? 2 : 8, CH = DP / 8, ST = L::STAGES;
-  pdl_enter_grid();
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
   __shared__ unsigned long long bad_keys;
-  const uint32_t q_s = smem_u32(smem), kv_s = q_s + L::Q_BYTES;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t* empty = full + ST;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + ST);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_enter_grid();
+  const uint32_t q_s = smem_u32(smem + L::Q_AT);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int kvh = blockIdx.y, split = blockIdx.z;
   const int hd = a.c.hd, rep = a.rep;
@@ -114,6 +122,50 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
   if (split > 0 && split >= cut.used) return;  // the join knows
   const int t_begin = cut.first + split * cut.per;
   const int t_end = min(min(t_begin + cut.per, cut.first + cut.tiles), (block_hi + TILE - 1) / TILE);
+  if (w == 4) {
+    const int32_t* table = a.c.table + static_cast<long long>(max(0, e.row)) * a.c.max_pages;
+    const int box = min(1 << a.c.ps_shift, TILE);
+    bool ok = true;
+    int t = t_begin;
+    for (; t < t_end; ++t) {
+      const int stage = (t - t_begin) % ST;
+      const uint32_t phase = static_cast<uint32_t>(((t - t_begin) / ST) & 1);
+      const int p = t * TILE + lane * box, boxes = (min(TILE, block_hi - t * TILE) + box - 1) / box;
+      int page = 0;
+      if (lane < boxes) {
+        page = table[p >> a.c.ps_shift];
+        if (page < 0 || page >= a.c.n_pages) {
+          atomicOr(a.c.status, ST_BAD_CACHE);
+          page = 0;
+        }
+      }
+      ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[stage], phase ^ 1u, abort_flag));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box * DP * 4);
+      __syncwarp();
+      if (lane < boxes) {
+        const uint32_t dst = smem_u32(smem + stage * 2 * L::KV) + lane * box * 128;
+        const int y = (kvh << a.c.ps_shift) + (p & ((1 << a.c.ps_shift) - 1));
+#pragma unroll
+        for (int h = 0; h < DP / 64; ++h) {
+          tma_3d(dst + h * L::HALF, &kmap, 64 * h, y, page, &full[stage]);
+          tma_3d(dst + L::KV + h * L::HALF, &vmap, 64 * h, y, page, &full[stage]);
+        }
+      }
+    }
+    if (lane == 0) {
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(a.c.status, ST_TIMEOUT_EMPTY);
+      }
+      bool drained = true;  // no copy may still be landing when the block exits
+      for (int x = max(t_begin, t - ST); x < t; ++x)
+        if (!mbar_wait(&full[(x - t_begin) % ST], static_cast<uint32_t>(((x - t_begin) / ST) & 1))) drained = false;
+      if (!drained) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
+    }
+    return;
+  }
+
   const int wr = WM == 4 ? w * 16 : 0;  // the warp's rows of the block
   int hi[2], tok[2], head[2];
 #pragma unroll
@@ -123,40 +175,25 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
     head[h] = kvh * rep + r % rep;
     hi[h] = e.row < 0 ? 0 : pre ? shared : e.len - e.nq + r / rep + 1;
   }
-
-  const uint16_t* kb = a.c.k + a.layer_off + (static_cast<long long>(kvh) << a.c.ps_shift) * hd;
-  const uint16_t* vb = a.c.v + a.layer_off + (static_cast<long long>(kvh) << a.c.ps_shift) * hd;
-  const int32_t* table = a.c.table + static_cast<long long>(max(0, e.row)) * a.c.max_pages;
-  auto load_tile = [&](int t, int stage) {
-    const uint32_t dst = kv_s + stage * 2 * L::KV_BYTES;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < TILE * CH; i += 128) {
-      const int key = i / CH, ch = i % CH, p = t * TILE + key;
-      const bool on = p >= e.start && p < block_hi && ch * 8 < hd;
-      long long off = 0;
-      bool ok = on;
-      if (on) {
-        const int page = table[p >> a.c.ps_shift];
-        ok = page >= 0 && page < a.c.n_pages;
-        if (!ok) atomicOr(a.c.status, ST_BAD_CACHE);
-        else off = page * a.c.page_stride + static_cast<long long>(p & ((1 << a.c.ps_shift) - 1)) * hd + ch * 8;
-      }
-      const uint32_t at = dst + key * DP * 2 + ((ch ^ (key & 7)) << 4);
-      cp16(at, kb + off, ok);
-      cp16(at + L::KV_BYTES, vb + off, ok);
-    }
-  };
-
-  for (int i = threadIdx.x; i < ROWS * CH; i += 128) {
-    const int r = i / CH, ch = i % CH, rr = r0 + min(r, n_rows - 1);
-    const long long at = (static_cast<long long>(e.t0 + rr / rep) * a.n_heads + kvh * rep + rr % rep) * hd + ch * 8;
-    cp16(q_s + r * DP * 2 + ((ch ^ (r & 7)) << 4), a.q + (ch * 8 < hd ? at : 0), ch * 8 < hd);
-  }
+  {
+    // a thread takes one chunk of eight elements of every (128 / CH)th row; rows past the end are the last
+    constexpr int EACH = ROWS * CH / 128, STEP = ROWS / EACH;
+    const int ch = threadIdx.x % CH;
+    uint4 v[EACH];
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s) {
-    if (t_begin + s < t_end) load_tile(t_begin + s, s);
-    cp_commit();
+    for (int x = 0; x < EACH; ++x) {
+      const int rr = r0 + min(static_cast<int>(threadIdx.x) / CH + x * STEP, n_rows - 1);
+      v[x] = ch * 8 < hd ? *reinterpret_cast<const uint4*>(
+                               a.q + (static_cast<long long>(e.t0 + rr / rep) * a.n_heads + kvh * rep + rr % rep) * hd + ch * 8)
+                         : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int x = 0; x < EACH; ++x) {
+      const int r = threadIdx.x / CH + x * STEP;
+      *reinterpret_cast<uint4*>(smem + L::Q_AT + r * DP * 2 + ((ch ^ (r & 7)) << 4)) = v[x];
+    }
   }
+  named_bar_sync(1, 128);
 
   float o[DP / 8][4];
 #pragma unroll
@@ -165,13 +202,15 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
   const int kw = WM == 1 ? w * 16 : 0;  // the warp's positions of a tile
   const int g = lane >> 3, lr = lane & 7;
 
+  // A given-up wait does not leave the loop: its barriers are all four warps'.  What follows it is void,
+  // and the status says so.
+  bool ok = true;
+  int stage = 0;
+  uint32_t phase = 0;
   for (int t = t_begin; t < t_end; ++t) {
-    const int stage = (t - t_begin) % ST;
-    cp_wait<ST - 2>();
-    __syncthreads();
-    if (t + ST - 1 < t_end) load_tile(t + ST - 1, (t - t_begin + ST - 1) % ST);
-    cp_commit();
-    const uint32_t ks = kv_s + stage * 2 * L::KV_BYTES, vs = ks + L::KV_BYTES;
+    ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&full[stage], phase, abort_flag));
+    uint8_t* vp = smem + stage * 2 * L::KV + L::KV;
+    const uint32_t ks = smem_u32(smem + stage * 2 * L::KV), vs = ks + L::KV;
 
     float s[NT][4];
 #pragma unroll
@@ -185,7 +224,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
       for (int i = 0; i < NT; i += 2) {
         uint32_t kf[4];
         const int key = kw + i * 8 + lr + (g >> 1) * 8, ch = 2 * kk + (g & 1);
-        ldsm4(kf, ks + key * DP * 2 + ((ch ^ (key & 7)) << 4));
+        ldsm4(kf, ks + (ch >> 3) * L::HALF + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
         mma16816<T>(s[i], qa, kf[0], kf[1]);
         mma16816<T>(s[i + 1], qa, kf[2], kf[3]);
       }
@@ -234,14 +273,14 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
       const int from = max(0, block_lo_hi - t * TILE), n = min(TILE, block_hi - t * TILE) - from;
       for (int x = threadIdx.x; x < n * CH; x += 128) {
         const int key = from + x / CH, ch = x % CH;
-        const uint4 v = *reinterpret_cast<const uint4*>(smem + (vs - q_s) + key * DP * 2 + ((ch ^ (key & 7)) << 4));
+        const uint4 v = *reinterpret_cast<const uint4*>(vp + (ch >> 3) * L::HALF + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
         if (!finite16<T>(v)) bad |= 1ull << key;
       }
-      if (__syncthreads_or(bad != 0)) {
-        if (threadIdx.x == 0) bad_keys = 0;
-        __syncthreads();
-        if (bad != 0) atomicOr(&bad_keys, bad);
-        __syncthreads();
+      if (threadIdx.x == 0) bad_keys = 0;
+      named_bar_sync(1, 128);
+      if (bad != 0) atomicOr(&bad_keys, bad);
+      named_bar_sync(1, 128);
+      if (bad_keys != 0) {
         bad = bad_keys;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -254,37 +293,71 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
               if (p >= hi[h]) continue;
 #pragma unroll
               for (int d = 0; d < DP / 8; ++d) {
-                const float2 v = unpack16<T>(*reinterpret_cast<const uint32_t*>(smem + (vs - q_s) + key * DP * 2 +
-                                                                                ((d ^ (key & 7)) << 4) + (lane & 3) * 4));
+                const float2 v = unpack16<T>(*reinterpret_cast<const uint32_t*>(
+                    vp + (d >> 3) * L::HALF + key * 128 + (((d & 7) ^ (key & 7)) << 4) + (lane & 3) * 4));
                 o[d][2 * h] += pr * v.x;
                 o[d][2 * h + 1] += pr * v.y;
               }
             }
           }
-        __syncthreads();
+        named_bar_sync(1, 128);
         for (int x = threadIdx.x; x < n * CH; x += 128) {
           const int key = from + x / CH, ch = x % CH;
-          if (((bad >> key) & 1) != 0) *reinterpret_cast<uint4*>(smem + (vs - q_s) + key * DP * 2 + (ch << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          if (((bad >> key) & 1) != 0) *reinterpret_cast<uint4*>(vp + (ch >> 3) * L::HALF + key * 128 + ((ch & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
         }
-        __syncthreads();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into it
+        named_bar_sync(1, 128);
       }
     }
+    // positions that are not the block's hold anything: their values count as 0
+    const bool edge = t * TILE < e.start || (t + 1) * TILE > block_hi;
 #pragma unroll
     for (int i = 0; i < NT; i += 2) {
-      const uint32_t pa[4] = {pack16<T>(s[i][0], s[i][1]), pack16<T>(s[i][2], s[i][3]), pack16<T>(s[i + 1][0], s[i + 1][1]),
-                              pack16<T>(s[i + 1][2], s[i + 1][3])};
+      uint32_t pa[4], rest[4], keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float p0v = s[i + (x >> 1)][2 * (x & 1)], p1v = s[i + (x >> 1)][2 * (x & 1) + 1];
+        if constexpr (WM == 1)
+          split16<T>(p0v, p1v, pa[x], rest[x]);
+        else
+          pa[x] = pack16<T>(p0v, p1v);
+      }
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int p = p0 + (i + x) * 8 + (lane & 3) * 2;
+          keep[x] = (p >= e.start && p < block_hi ? 0xFFFFu : 0u) | (p + 1 >= e.start && p + 1 < block_hi ? 0xFFFF0000u : 0u);
+        }
+      }
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
         uint32_t vf[4];
         const int key = kw + i * 8 + lr + (g & 1) * 8, ch = 2 * d + (g >> 1);
-        ldsm4t(vf, vs + key * DP * 2 + ((ch ^ (key & 7)) << 4));
+        ldsm4t(vf, vs + (ch >> 3) * L::HALF + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
+        vf[0] &= keep[0];
+        vf[1] &= keep[1];
+        vf[2] &= keep[0];
+        vf[3] &= keep[1];
         mma16816<T>(o[2 * d], pa, vf[0], vf[1]);
         mma16816<T>(o[2 * d + 1], pa, vf[2], vf[3]);
+        if constexpr (WM == 1) {
+          mma16816<T>(o[2 * d], rest, vf[0], vf[1]);
+          mma16816<T>(o[2 * d + 1], rest, vf[2], vf[3]);
+        }
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);
+    if (++stage == ST) {
+      stage = 0;
+      phase ^= 1u;
+    }
   }
-  cp_wait<0>();
-  __syncthreads();
+  if (!ok && lane == 0) {
+    *abort_flag = 1;
+    atomicOr(a.c.status, ST_TIMEOUT_FULL);
+  }
+  named_bar_sync(1, 128);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
@@ -312,7 +385,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
   } else {
     // join the four warps' positions: their m and l, then their sums through shared memory
     __shared__ float2 ml_s[4][16];
-    float* o_s = reinterpret_cast<float*>(smem + L::Q_BYTES);
+    float* o_s = reinterpret_cast<float*>(smem);
     if ((lane & 3) == 0) {
       ml_s[w][lane >> 2] = make_float2(m[0], l[0]);
       ml_s[w][(lane >> 2) + 8] = make_float2(m[1], l[1]);
@@ -323,7 +396,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<float2*>(o_s + (w * 16 + (lane >> 2) + 8 * h) * DP + i * 8 + (lane & 3) * 2) =
             make_float2(o[i][2 * h], o[i][2 * h + 1]);
-    __syncthreads();
+    named_bar_sync(1, 128);
     for (int x = threadIdx.x; x < n_rows * (DP / 2); x += 128) {
       const int r = x / (DP / 2), d = x % (DP / 2) * 2;
       float mm = -INFINITY;
@@ -353,109 +426,118 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, const 
   }
 }
 
-// Parts of the shared pass that a token's head has.
-__device__ __forceinline__ int tc_parts(const AttnArgs& a, int shared, int t, int head) {
-  const TcCut c = tc_cut(a, shared);
-  const int kvh = head / a.rep, r = t * a.rep + head - kvh * a.rep;
-  const long long first = (static_cast<long long>(kvh) * c.row_blocks + r / a.pre_rows) * c.tiles;
-  return static_cast<int>((first + c.tiles - 1) / c.per - first / c.per) + 1;
-}
-
-// Join the parts of each (token, head): a warp a row, lane x has elements 4 x ... and 4 x + 128 ...  The
-// parts' weights come first, a lane a part, then their sums eight at a time.
-template <typename T>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+// Join the parts of each (token, head): a warp takes `heads` heads of a token, lane x elements 4 x ... and,
+// in wide heads, 4 x + 128 ...  The parts' weights come first, a lane a part, then their sums four at a time.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const int heads, const int per_token) {
   pdl_enter_grid();
-  const int lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<long long>(a.n_tokens) * a.n_heads) return;
-  const int t = static_cast<int>(row / a.n_heads), head = static_cast<int>(row - static_cast<long long>(t) * a.n_heads), hd = a.c.hd;
+  const int lane = threadIdx.x & 31, hd = a.c.hd;
+  const int unit = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5), t = unit / per_token;
+  if (t >= a.n_tokens) return;
   int i = t;
-  if (a.q_start != nullptr) {  // the last entry that starts at or before t
-    int lo = 0, up = a.n_batch;
-    while (up - lo > 1) {
-      const int mid = (lo + up) / 2;
-      if (a.q_start[mid] <= t) lo = mid;
-      else up = mid;
+  if (a.q_start != nullptr) {  // the last entry that starts at or before t: 32 of them at a time
+    i = 0;
+    for (int base = 0; base < a.n_batch; base += 32) {
+      const bool at = base + lane < a.n_batch && a.q_start[base + lane] <= t;
+      const uint32_t m = __ballot_sync(0xFFFFFFFFu, at);
+      if (m != 0) i = base + 31 - __clz(m);
+      if (m != 0xFFFFFFFFu) break;
     }
-    i = lo;
   }
   const int shared = shared_of(a);
   const Entry e = entry_of(a, i, shared);
   const bool sees = e.row >= 0 && t >= e.t0 && t < e.t0 + e.nq && e.len - e.nq + (t - e.t0) + 1 > 0;
-  int n_pre = 0, n_own = 0;
-  long long cont = 0;  // single tokens: the row of the second own part
-  if (sees) {
-    if (e.shares) n_pre = a.pre_rows > 0 ? tc_parts(a, shared, t, head) : cut_of(0, shared, a.n_pre).used;
-    if (a.own_ctas > 0) {
-      const int tiles = cut_of(e.start, e.len, 1).tiles;
-      if (tiles > 0) {
-        const int kvh = head / a.rep, r = head - kvh * a.rep, n_rb = (a.rep + 15) / 16, per_entry = a.c.n_kv * n_rb;
-        const long long per = (static_cast<long long>(a.own_off[a.n_batch]) * per_entry + a.own_ctas - 1) / a.own_ctas;
-        const long long first = static_cast<long long>(a.own_off[i]) * per_entry + static_cast<long long>(kvh * n_rb + r / 16) * tiles;
-        const int c0 = static_cast<int>(first / per);
-        n_own = static_cast<int>((first + tiles - 1) / per) - c0 + 1;
-        cont = a.cont_row0 + static_cast<long long>(c0 + 1) * 16 + r % 16;
-      }
-    } else {
-      n_own = cut_of(e.start, e.len, a.n_own).used;
-    }
+  const int own_tiles = sees && a.own_ctas > 0 ? cut_of(e.start, e.len, 1).tiles : 0;
+  const int n_rb = (a.rep + 15) / 16, per_entry = a.c.n_kv * n_rb;
+  long long own_per = 1, own_first = 0;
+  if (own_tiles > 0) {
+    own_per = (static_cast<long long>(a.own_off[a.n_batch]) * per_entry + a.own_ctas - 1) / a.own_ctas;
+    own_first = static_cast<long long>(a.own_off[i]) * per_entry;
   }
+  const int own_slots = sees && a.own_ctas == 0 ? cut_of(e.start, e.len, a.n_own).used : 0;
+  const TcCut pre = sees && e.shares && a.pre_rows > 0 ? tc_cut(a, shared) : TcCut{1, 1, 1, 1};
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
-  const int n = n_pre + n_own;
-  auto row_of = [&](int x) {
-    if (x < n_pre) return x * rows + row;
-    x -= n_pre;
-    return a.own_ctas > 0 && x > 0 ? cont + 16LL * (x - 1) : (a.n_pre + x) * rows + row;
-  };
-  float top = -INFINITY, l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  for (int b = 0; b < n; b += 32) {
-    const float2 ml = b + lane < n ? a.part_ml[row_of(b + lane)] : make_float2(-INFINITY, 0.0f);
-    float most = ml.x;
-#pragma unroll
-    for (int y = 16; y > 0; y >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, y));
-    const float before = top;
-    top = fmaxf(top, most);
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float f = exp2f(ml.x - base), g = exp2f(before - base);
-    float lw = f * ml.y;
-#pragma unroll
-    for (int y = 16; y > 0; y >>= 1) lw += __shfl_xor_sync(0xFFFFFFFFu, lw, y);
-    l = l * g + lw;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] *= g;
-    const bool none = ml.x == -INFINITY && ml.y == 0.0f;  // nothing seen: its sums may not be written
-    for (int x0 = 0; x0 < min(32, n - b); x0 += 8) {
-      float4 v[8][2];
-      float w[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        w[x] = __shfl_sync(0xFFFFFFFFu, f, x0 + x);
-        const bool skip = __shfl_sync(0xFFFFFFFFu, static_cast<int>(none), x0 + x) != 0;
-        const float* src = a.part_o + row_of(b + x0 + x) * hd;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int d = lane * 4 + k * 128;
-          v[x][k] = !skip && d < hd ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
+
+  const int h0 = (unit - t * per_token) * heads;
+  for (int head = h0; head < min(h0 + heads, a.n_heads); ++head) {
+    const int kvh = head / a.rep, r = head - kvh * a.rep;
+    const long long row = static_cast<long long>(t) * a.n_heads + head;
+    int n_pre = 0, n_own = own_slots;
+    long long cont = 0;  // single tokens: the row of the second own part
+    if (sees && e.shares) {
+      if (a.pre_rows > 0) {
+        const int first = (kvh * pre.row_blocks + (t * a.rep + r) / a.pre_rows) * pre.tiles;
+        n_pre = (first + pre.tiles - 1) / pre.per - first / pre.per + 1;
+      } else {
+        n_pre = cut_of(0, shared, a.n_pre).used;
       }
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          o[4 * k] += w[x] * v[x][k].x;
-          o[4 * k + 1] += w[x] * v[x][k].y;
-          o[4 * k + 2] += w[x] * v[x][k].z;
-          o[4 * k + 3] += w[x] * v[x][k].w;
-        }
     }
-  }
+    if (own_tiles > 0) {
+      const long long first = own_first + static_cast<long long>(kvh * n_rb + r / 16) * own_tiles;
+      const int c0 = static_cast<int>(first / own_per);
+      n_own = static_cast<int>((first + own_tiles - 1) / own_per) - c0 + 1;
+      cont = a.cont_row0 + static_cast<long long>(c0 + 1) * 16 + r % 16;
+    }
+    const int n = n_pre + n_own;
+    auto row_of = [&](int x) {
+      if (x < n_pre) return x * rows + row;
+      x -= n_pre;
+      return a.own_ctas > 0 && x > 0 ? cont + 16LL * (x - 1) : (a.n_pre + x) * rows + row;
+    };
+    float top = -INFINITY, l = 0.0f;
+    float4 o[WIDE ? 2 : 1];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int d = lane * 4 + k * 128;
-    if (d < hd) {
-      store_out<T>(a, row * hd + d, o[4 * k], o[4 * k + 1], l, sees);
-      store_out<T>(a, row * hd + d + 2, o[4 * k + 2], o[4 * k + 3], l, sees);
+    for (int k = 0; k < (WIDE ? 2 : 1); ++k) o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int b = 0; b < n; b += 32) {
+      const float2 ml = b + lane < n ? a.part_ml[row_of(b + lane)] : make_float2(-INFINITY, 0.0f);
+      float most = ml.x;
+#pragma unroll
+      for (int y = 16; y > 0; y >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, y));
+      const float before = top;
+      top = fmaxf(top, most);
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float f = exp2f(ml.x - base), g = exp2f(before - base);
+      float lw = f * ml.y;
+#pragma unroll
+      for (int y = 16; y > 0; y >>= 1) lw += __shfl_xor_sync(0xFFFFFFFFu, lw, y);
+      l = l * g + lw;
+#pragma unroll
+      for (int k = 0; k < (WIDE ? 2 : 1); ++k) o[k] = make_float4(o[k].x * g, o[k].y * g, o[k].z * g, o[k].w * g);
+      // a part that saw nothing may not have written its sums
+      uint32_t some = __ballot_sync(0xFFFFFFFFu, ml.x != -INFINITY || ml.y != 0.0f);
+      while (some != 0) {
+        float4 v[4][WIDE ? 2 : 1];
+        float w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int part = some != 0 ? __ffs(some) - 1 : -1;
+          w[x] = __shfl_sync(0xFFFFFFFFu, f, max(part, 0));
+          const float* src = a.part_o + row_of(b + max(part, 0)) * hd + lane * 4;
+#pragma unroll
+          for (int k = 0; k < (WIDE ? 2 : 1); ++k)
+            v[x][k] = part >= 0 && lane * 4 + k * 128 < hd ? *reinterpret_cast<const float4*>(src + k * 128)
+                                                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (part < 0) w[x] = 0.0f;
+          some &= some - 1;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int k = 0; k < (WIDE ? 2 : 1); ++k) {
+            o[k].x += w[x] * v[x][k].x;
+            o[k].y += w[x] * v[x][k].y;
+            o[k].z += w[x] * v[x][k].z;
+            o[k].w += w[x] * v[x][k].w;
+          }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < (WIDE ? 2 : 1); ++k) {
+      const int d = lane * 4 + k * 128;
+      if (d < hd) {
+        store_out<T>(a, row * hd + d, o[k].x, o[k].y, l, sees);
+        store_out<T>(a, row * hd + d + 2, o[k].z, o[k].w, l, sees);
+      }
     }
   }
 }
@@ -497,7 +579,7 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
     p.n_own = static_cast<int>(std::max(1LL, std::min({(target + at_once - 1) / at_once, static_cast<long long>((own_tiles + 1) / 2),
                                                       static_cast<long long>(MAX_SLOTS)})));
   }
-  if (shared_len > 0 && hd <= 128 && rows > 16) {
+  if (shared_len > 0 && hd <= 128 && rows > 16 && (rows + 255) / 128 * n_kv * ((shared_len + TC_TILE - 1) / TC_TILE) < INT_MAX) {
     const int tiles = (shared_len + TC_TILE - 1) / TC_TILE;
     p.pre_rows = rows > 128 ? 256 : 128;
     const long long blocks = (rows + p.pre_rows - 1) / p.pre_rows * n_kv;
@@ -528,23 +610,26 @@ size_t work_bytes(const AttnPlan& p, int n_batch, int n_tokens, int n_heads, int
 }
 
 template <typename T, int DP, int WM>
-cudaError_t launch_rows_as(const AttnArgs& a, int blocks, int splits, int pre, cudaStream_t st) {
+cudaError_t launch_rows_as(const AttnArgs& a, uint32_t type, int blocks, int splits, int pre, cudaStream_t st) {
   using L = RowsLayout<DP, WM>;
   static const cudaError_t set =
       cudaFuncSetAttribute(attn_rows_kernel<T, DP, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
   if (set != cudaSuccess) return set;
-  return launch_dependent(attn_rows_kernel<T, DP, WM>, dim3(blocks, a.c.n_kv, splits), dim3(128), L::ALLOC, st, a, pre);
+  CUtensorMap kmap, vmap;
+  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type, TILE) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type, TILE))
+    return cudaErrorInvalidValue;
+  return launch_dependent(attn_rows_kernel<T, DP, WM>, dim3(blocks, a.c.n_kv, splits), dim3(ROWS_THREADS), L::ALLOC, st, a, kmap, vmap, pre);
 }
 
 template <typename T>
-cudaError_t launch_rows(const AttnArgs& a, int wm, int blocks, int splits, int pre, cudaStream_t st) {
+cudaError_t launch_rows(const AttnArgs& a, uint32_t type, int wm, int blocks, int splits, int pre, cudaStream_t st) {
   if (wm == 1)
-    return a.c.hd <= 64    ? launch_rows_as<T, 64, 1>(a, blocks, splits, pre, st)
-           : a.c.hd <= 128 ? launch_rows_as<T, 128, 1>(a, blocks, splits, pre, st)
-                           : launch_rows_as<T, 256, 1>(a, blocks, splits, pre, st);
-  return a.c.hd <= 64    ? launch_rows_as<T, 64, 4>(a, blocks, splits, pre, st)
-         : a.c.hd <= 128 ? launch_rows_as<T, 128, 4>(a, blocks, splits, pre, st)
-                         : launch_rows_as<T, 256, 4>(a, blocks, splits, pre, st);
+    return a.c.hd <= 64    ? launch_rows_as<T, 64, 1>(a, type, blocks, splits, pre, st)
+           : a.c.hd <= 128 ? launch_rows_as<T, 128, 1>(a, type, blocks, splits, pre, st)
+                           : launch_rows_as<T, 256, 1>(a, type, blocks, splits, pre, st);
+  return a.c.hd <= 64    ? launch_rows_as<T, 64, 4>(a, type, blocks, splits, pre, st)
+         : a.c.hd <= 128 ? launch_rows_as<T, 128, 4>(a, type, blocks, splits, pre, st)
+                         : launch_rows_as<T, 256, 4>(a, type, blocks, splits, pre, st);
 }
 
 template <typename T>
@@ -553,13 +638,17 @@ cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, uint32_t t
     const cudaError_t e = launch_attn_tc(a, type, st);
     if (e != cudaSuccess) return e;
   } else if (p.n_pre > 0) {
-    const cudaError_t e = launch_rows<T>(a, p.pre_wm, p.pre_blocks, p.n_pre, 1, st);
+    const cudaError_t e = launch_rows<T>(a, type, p.pre_wm, p.pre_blocks, p.n_pre, 1, st);
     if (e != cudaSuccess) return e;
   }
-  const cudaError_t e = p.one ? launch_attn_one(a, type, st) : launch_rows<T>(a, p.own_wm, p.own_blocks, p.n_own, 0, st);
+  const cudaError_t e = p.one ? launch_attn_one(a, type, st) : launch_rows<T>(a, type, p.own_wm, p.own_blocks, p.n_own, 0, st);
   if (e != cudaSuccess || part_rows(p, a.n_tokens, a.n_heads) == 0) return e;
+  // a head a warp while that leaves warps free, else several: what a token needs is looked up once for them
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
-  return launch_dependent(attn_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, st, a);
+  const int heads = rows <= 32LL * api_device_info().sm_count ? 1 : 4, per_token = (a.n_heads + heads - 1) / heads;
+  const unsigned blocks = static_cast<unsigned>((static_cast<long long>(a.n_tokens) * per_token + 3) / 4);
+  return launch_dependent(a.c.hd > 128 ? attn_join_kernel<T, true> : attn_join_kernel<T, false>, dim3(blocks), dim3(128), 0, st, a,
+                          heads, per_token);
 }
 
 }  // namespace

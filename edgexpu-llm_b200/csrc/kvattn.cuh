@@ -95,14 +95,13 @@ __device__ __forceinline__ Cut cut_of(int start, int end, int n) {
 // divided over the pieces that touch it, and piece c's part of it is slot c - (the first such piece).
 constexpr int TC_TILE = 128;  // positions
 struct TcCut {
-  int tiles, row_blocks;
-  long long total, per;
+  int tiles, row_blocks, total, per;
 };
 __device__ __forceinline__ TcCut tc_cut(const AttnArgs& a, int shared) {
   TcCut c;
   c.tiles = (shared + TC_TILE - 1) / TC_TILE;
   c.row_blocks = (a.n_tokens * a.rep + a.pre_rows - 1) / a.pre_rows;
-  c.total = static_cast<long long>(c.row_blocks) * a.c.n_kv * c.tiles;
+  c.total = c.row_blocks * a.c.n_kv * c.tiles;
   c.per = (c.total + a.pre_ctas - 1) / a.pre_ctas;
   return c;
 }

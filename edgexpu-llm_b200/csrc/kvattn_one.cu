@@ -292,15 +292,22 @@ __global__ void __launch_bounds__(ONE_THREADS)
               s[n][x] = ex2(s[n][x] - ((mm == -INFINITY ? 0.0f : mm) - P_SHIFT));
               l[x >> 1] += s[n][x];
             }
-          const uint32_t pa[4] = {pack16<T>(s[0][0], s[0][1]), pack16<T>(s[0][2], s[0][3]), pack16<T>(s[1][0], s[1][1]),
-                                  pack16<T>(s[1][2], s[1][3])};
+          uint32_t pa[4], rest[4];  // P in two numbers of the type: bytes bound here, not products
+#pragma unroll
+          for (int x = 0; x < 4; ++x) split16<T>(s[x >> 1][2 * (x & 1)], s[x >> 1][2 * (x & 1) + 1], pa[x], rest[x]);
 #pragma unroll
           for (int d = 0; d < DP / 16; ++d) {
             uint32_t vf[4];
             const int key = kw + lr + (g & 1) * 8, ch = 2 * d + (g >> 1);
             ldsm4t(vf, vs + (ch >> 3) * L::HALF + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
-            mma16816<T>(o[2 * d], pa, vf[0] & keep[0], vf[1] & keep[1]);
-            mma16816<T>(o[2 * d + 1], pa, vf[2] & keep[0], vf[3] & keep[1]);
+            vf[0] &= keep[0];
+            vf[1] &= keep[1];
+            vf[2] &= keep[0];
+            vf[3] &= keep[1];
+            mma16816<T>(o[2 * d], pa, vf[0], vf[1]);
+            mma16816<T>(o[2 * d + 1], pa, vf[2], vf[3]);
+            mma16816<T>(o[2 * d], rest, vf[0], vf[1]);
+            mma16816<T>(o[2 * d + 1], rest, vf[2], vf[3]);
           }
         }
         __syncwarp();

@@ -27,9 +27,6 @@ namespace ex {
 namespace {
 
 constexpr int TC_THREADS = 384;
-#ifndef POLY_OF_8
-#define POLY_OF_8 0
-#endif
 
 template <int DP, int MT>
 struct TcLayout {
@@ -137,26 +134,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// 2^x of a pair without the special-function units, for x <= 16: x = n + f with n the nearest integer
-// (found in the low bits of x + 1.5 2^23), 2^f by the minimax polynomial of degree 4 on [-1/2, 1/2] with
-// value 1 at 0 (Remez exchange; relative error 3.6e-6, below the weights' rounding to 11 bits), and n
-// added to the exponent.  At and below -127 the result is 0.  A NaN is not kept.
-__device__ __forceinline__ float2 exp2_poly(f32x2 x) {
-  constexpr float MAGIC = 12582912.0f;
-  const float2 c = one_by_one(x);
-  x = two(fmaxf(c.x, -127.0f), fmaxf(c.y, -127.0f));
-  const f32x2 t = add2(x, two(MAGIC, MAGIC));
-  const f32x2 f = add2(x, fma2(t, two(-1.0f, -1.0f), two(MAGIC, MAGIC)));
-  f32x2 p = two(0.009782912f, 0.009782912f);
-  p = fma2(p, f, two(0.055976883f, 0.055976883f));
-  p = fma2(p, f, two(0.24020711f, 0.24020711f));
-  p = fma2(p, f, two(0.69311362f, 0.69311362f));
-  p = fma2(p, f, two(1.0f, 1.0f));
-  const float2 n = one_by_one(t), v = one_by_one(p);
-  return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(n.x) << 23)),
-                     __int_as_float(__float_as_int(v.y) + (__float_as_int(n.y) << 23)));
-}
-
 __device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
@@ -194,14 +171,14 @@ struct Segment {
   int kvh, row0, tile0, n, slot;
   int steps;  // the prefix's last half tile may be empty
 };
-__device__ __forceinline__ Segment segment_at(const TcCut& c, long long at, long long end, int pre_rows, int shared) {
+__device__ __forceinline__ Segment segment_at(const TcCut& c, int at, int end, int pre_rows, int shared) {
   Segment s;
-  const long long block = at / c.tiles;
-  s.tile0 = static_cast<int>(at - block * c.tiles);
-  s.n = static_cast<int>(min(static_cast<long long>(c.tiles - s.tile0), end - at));
-  s.kvh = static_cast<int>(block / c.row_blocks);
-  s.row0 = static_cast<int>(block - static_cast<long long>(s.kvh) * c.row_blocks) * pre_rows;
-  s.slot = static_cast<int>(blockIdx.x - block * c.tiles / c.per);
+  const int block = at / c.tiles;
+  s.tile0 = at - block * c.tiles;
+  s.n = min(c.tiles - s.tile0, end - at);
+  s.kvh = block / c.row_blocks;
+  s.row0 = (block - s.kvh * c.row_blocks) * pre_rows;
+  s.slot = static_cast<int>(blockIdx.x) - block * c.tiles / c.per;
   s.steps = min(2 * s.n, (shared - s.tile0 * TC_TILE + STEP - 1) / STEP);
   return s;
 }
@@ -261,7 +238,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   const int shared = __shfl_sync(0xFFFFFFFFu, shared_of(a), 0);
   const TcCut cut = tc_cut(a, shared);
-  const long long begin = blockIdx.x * cut.per, end = min(cut.total, begin + cut.per);
+  const int begin = min(cut.total, static_cast<int>(blockIdx.x) * cut.per), end = min(cut.total, begin + cut.per);
 
   if (warp == 0) {
     // K of tile 0, V of tile 0, K of tile 1, ...: the order in which the products need them
@@ -270,7 +247,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     Ring<NS> ring;
     int issued = 0;  // slots filled, NS at most
     bool ok = true;
-    for (long long at = begin; ok && at < end;) {
+    for (int at = begin; ok && at < end;) {
       const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
       for (int i = 0; ok && i < g.n; ++i) {
@@ -333,7 +310,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
       tc_commit(&s_full[2 * half + b]);
     };
-    for (long long at = begin; ok && at < end; ++segs) {
+    for (int at = begin; ok && at < end; ++segs) {
       const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
       Ring<NS> k = v;
@@ -356,7 +333,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int j = 0; ok && j < g.steps; j += 2) {
         k.next();
         k.next();
-        ok = there(&full[v.slot], v.phase) && (j + 2 >= g.steps || there(&full[k.slot], k.phase));
+        ok = there(&full[v.slot], v.phase);
         const uint32_t kd = sw128_desc(ring_s + k.slot * L::SLOT, 16), vd0 = sw128_desc(ring_s + v.slot * L::SLOT, L::HALF);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -376,8 +353,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
               }
               tc_commit(&o_done[2 * h + b]);
-              if (more) product_s(h, kd, b);
             }
+            __syncwarp();
+            if (more && b == 0 && h == 0) ok = there(&full[k.slot], k.phase);
+            if (!ok) break;
+            if (more && lead) product_s(h, kd, b);
             __syncwarp();
           }
           par[b] ^= 1u;
@@ -411,7 +391,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     Ring<NS> ring;  // V of the tile in use
     ring.next();
     bool ok = true;
-    for (long long at = begin; ok && at < end; ++segs) {
+    for (int at = begin; ok && at < end; ++segs) {
       const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
       const int base_row = g.row0 + half * 128;
@@ -512,19 +492,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
         for (int c = 0; c < STEP; c += 2) {
           const f32x2 x = fma2(two(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, base2);
-          float2 p;
-          if ((c / 2) % 8 < POLY_OF_8) {
-            p = exp2_poly(x);
-          } else {
-            const float2 y = one_by_one(x);
-            p = make_float2(ex2(y.x), ex2(y.y));
-          }
+          const float2 y = one_by_one(x), p = make_float2(ex2(y.x), ex2(y.y));
           sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], two(p.x, p.y));
-          s[c >> 1] = pack16<T>(p.x, p.y);
-          if constexpr (FINE) {
-            const float2 h = unpack16<T>(s[c >> 1]);
-            rest[c >> 1] = pack16<T>(p.x - h.x, p.y - h.y);
-          }
+          if constexpr (FINE)
+            split16<T>(p.x, p.y, s[c >> 1], rest[c >> 1]);
+          else
+            s[c >> 1] = pack16<T>(p.x, p.y);
         }
         tc_st32(s_at, s);
         if constexpr (FINE) tc_st32(s_at + STEP / 2, rest);

@@ -228,6 +228,19 @@ def test_infinities_and_nan_of_the_data(kv):
         assert bool(((got.double() - want).abs() <= (u + 2.0 ** -15) * size + u * want.abs())[fine].all())
         if n_q is not None:
             assert not want[1:6].isnan().any() and want[8:13].isnan().any()
+    # in the prefix too, with few rows and with many
+    for batch in (1, 3, 20, 90):
+        cache = make(kv, [210] * batch, 200, 4, 2, 64, 16, torch.float16)
+        t = cache.table.long()
+        for x, value in ((7, float("inf")), (50, float("-inf")), (199, float("inf"))):
+            cache.v[0, t[0, x // 16], 0, x % 16, x % 61] = value
+        cache.v[0, t[1:, 199 // 16], 0, 199 % 16, 199 % 61] = float("inf")  # the copies of the page it shares in part
+        cache.k[0, t[0, 3], 1, 2, 4] = float("nan")
+        q = torch.randn(batch, 4, 64, device="cuda").half()
+        got = cache.attention(0, q, ints(*range(1, batch + 1)), shared_len=200)
+        want, _ = reference(cache, 0, q, list(range(1, batch + 1)), list(range(batch + 1)), 0.125)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf())
+        assert torch.equal(got.isneginf(), want.isneginf()) and want.isinf().any() and want.isfinite().any()
     # a row all of whose scores are -inf is 0/0
     cache = make(kv, [40], 0, 1, 1, 64, 16, torch.float16)
     cache.k[0, cache.table[1, :3].long()] = float("-inf")
