@@ -107,6 +107,20 @@ __device__ __forceinline__ void pdl_enter_grid() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// The same where the next grid runs beside this one: what came before is complete first, so that the next
+// grid need not wait for it.  That grid, in turn, waits for this one before it ends.
+__device__ __forceinline__ void pdl_enter_pair() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename F>
+cudaError_t allow_smem(F* kern, size_t bytes) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
+
 template <typename... KArgs, typename... Args>
 cudaError_t launch_dependent(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg{};

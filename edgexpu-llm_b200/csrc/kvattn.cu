@@ -30,14 +30,14 @@ constexpr int ROWS_THREADS = 160;
 template <int DP, int WM>
 struct RowsLayout {
   static constexpr int ROWS = 16 * WM;
-  static constexpr int STAGES = DP == 64 ? 3 : 2;
+  static constexpr int SLOTS = DP == 64 ? 6 : 3;
   static constexpr int HALF = TILE * 128;
-  static constexpr int KV = HALF * (DP / 64);  // a tile of K, or of V
-  static constexpr int Q_AT = STAGES * 2 * KV;
+  static constexpr int SLOT = HALF * (DP / 64);  // a tile of K, or of V
+  static constexpr int Q_AT = SLOTS * SLOT;
   static constexpr int BARS = Q_AT + ROWS * DP * 2;
   static constexpr int JOIN_BYTES = WM == 1 ? 4 * 16 * DP * 4 : 0;  // over the ring, when it is done with
-  static constexpr int ALLOC = BARS + 16 * STAGES + 64 + 1024;
-  static_assert(JOIN_BYTES <= STAGES * 2 * KV, "the join fits the ring");
+  static constexpr int ALLOC = BARS + 16 * SLOTS + 64 + 1024;
+  static_assert(JOIN_BYTES <= SLOTS * SLOT, "the join fits the ring");
 };
 
 // One block: 16 * WM rows of one key/value head against one part of the prefix (PRE) or of an entry's
@@ -47,10 +47,10 @@ struct RowsLayout {
 // product, as the tensor cores take it (with WM = 1, where bytes bound, in two numbers of the type); its
 // sum l is of the unrounded values.
 template <typename T, int DP, int WM>
-__global__ void __launch_bounds__(ROWS_THREADS)
+__global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
     attn_rows_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const int pre) {
   using L = RowsLayout<DP, WM>;
-  constexpr int ROWS = L::ROWS, NT = WM == 1 ? 2 : 8, CH = DP / 8, ST = L::STAGES;
+  constexpr int ROWS = L::ROWS, NT = WM == 1 ? 2 : 8, CH = DP / 8, ST = L::SLOTS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ unsigned long long bad_keys;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -66,7 +66,10 @@ __global__ void __launch_bounds__(ROWS_THREADS)
     fence_mbar_init();
   }
   __syncthreads();
-  pdl_enter_grid();
+  if (pre)
+    pdl_enter_pair();
+  else
+    own_enter(a);
   const uint32_t q_s = smem_u32(smem + L::Q_AT);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int kvh = blockIdx.y, split = blockIdx.z;
@@ -104,14 +107,20 @@ __global__ void __launch_bounds__(ROWS_THREADS)
         }
         before += __shfl_sync(0xFFFFFFFFu, inc, 31);
       }
-      if (found < 0) return;
+      if (found < 0) {
+        own_leave(a);
+        return;
+      }
       i = found;
     }
     e = entry_of(a, i, shared);
     r0 = blk * ROWS;
   }
   const int n_rows = min(ROWS, e.nq * rep - r0);
-  if (n_rows <= 0) return;
+  if (n_rows <= 0) {
+    if (!pre) own_leave(a);
+    return;
+  }
   const bool whole = a.n_pre + a.n_own == 1;  // the only part there is: no join follows
 
   // what the rows see: row r is token r / rep; rows past the end see what the last one does
@@ -119,49 +128,31 @@ __global__ void __launch_bounds__(ROWS_THREADS)
   const int block_hi = e.row < 0 ? 0 : pre ? shared : max(0, e.len - e.nq + last_tok + 1);
   const int block_lo_hi = e.row < 0 ? 0 : pre ? shared : max(0, e.len - e.nq + first_tok + 1);
   const Cut cut = pre ? cut_of(0, shared, a.n_pre) : cut_of(e.start, e.row < 0 ? 0 : e.len, a.n_own);
-  if (split > 0 && split >= cut.used) return;  // the join knows
+  if (split > 0 && split >= cut.used) {  // the join knows
+    if (!pre) own_leave(a);
+    return;
+  }
   const int t_begin = cut.first + split * cut.per;
   const int t_end = min(min(t_begin + cut.per, cut.first + cut.tiles), (block_hi + TILE - 1) / TILE);
   if (w == 4) {
     const int32_t* table = a.c.table + static_cast<long long>(max(0, e.row)) * a.c.max_pages;
-    const int box = min(1 << a.c.ps_shift, TILE);
+    Ring<ST> ring;
+    int issued = 0;
     bool ok = true;
-    int t = t_begin;
-    for (; t < t_end; ++t) {
-      const int stage = (t - t_begin) % ST;
-      const uint32_t phase = static_cast<uint32_t>(((t - t_begin) / ST) & 1);
-      const int p = t * TILE + lane * box, boxes = (min(TILE, block_hi - t * TILE) + box - 1) / box;
-      int page = 0;
-      if (lane < boxes) {
-        page = table[p >> a.c.ps_shift];
-        if (page < 0 || page >= a.c.n_pages) {
-          atomicOr(a.c.status, ST_BAD_CACHE);
-          page = 0;
-        }
-      }
-      ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[stage], phase ^ 1u, abort_flag));
+    for (int t = 2 * t_begin; t < 2 * t_end; ++t) {  // K of a tile, then its V
+      ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
       if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box * DP * 4);
-      __syncwarp();
-      if (lane < boxes) {
-        const uint32_t dst = smem_u32(smem + stage * 2 * L::KV) + lane * box * 128;
-        const int y = (kvh << a.c.ps_shift) + (p & ((1 << a.c.ps_shift) - 1));
-#pragma unroll
-        for (int h = 0; h < DP / 64; ++h) {
-          tma_3d(dst + h * L::HALF, &kmap, 64 * h, y, page, &full[stage]);
-          tma_3d(dst + L::KV + h * L::HALF, &vmap, 64 * h, y, page, &full[stage]);
-        }
-      }
+      bring_tile<DP, TILE>(a.c, table, (t & 1) == 0 ? &kmap : &vmap, smem_u32(smem + ring.slot * L::SLOT), kvh, (t >> 1) * TILE, block_hi,
+                     &full[ring.slot]);
+      issued = min(issued + 1, ST);
+      ring.next();
     }
     if (lane == 0) {
       if (!ok) {
         *abort_flag = 1;
         atomicOr(a.c.status, ST_TIMEOUT_EMPTY);
       }
-      bool drained = true;  // no copy may still be landing when the block exits
-      for (int x = max(t_begin, t - ST); x < t; ++x)
-        if (!mbar_wait(&full[(x - t_begin) % ST], static_cast<uint32_t>(((x - t_begin) / ST) & 1))) drained = false;
-      if (!drained) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
+      drain<ST>(ring, issued, full, a.c.status);
     }
     return;
   }
@@ -205,12 +196,14 @@ __global__ void __launch_bounds__(ROWS_THREADS)
   // A given-up wait does not leave the loop: its barriers are all four warps'.  What follows it is void,
   // and the status says so.
   bool ok = true;
-  int stage = 0;
-  uint32_t phase = 0;
+  Ring<ST> ring;
   for (int t = t_begin; t < t_end; ++t) {
-    ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&full[stage], phase, abort_flag));
-    uint8_t* vp = smem + stage * 2 * L::KV + L::KV;
-    const uint32_t ks = smem_u32(smem + stage * 2 * L::KV), vs = ks + L::KV;
+    ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
+    const uint32_t ks = smem_u32(smem + ring.slot * L::SLOT);
+    const int k_slot = ring.slot;
+    ring.next();
+    uint8_t* vp = smem + ring.slot * L::SLOT;
+    const uint32_t vs = smem_u32(vp);
 
     float s[NT][4];
 #pragma unroll
@@ -229,6 +222,8 @@ __global__ void __launch_bounds__(ROWS_THREADS)
         mma16816<T>(s[i + 1], qa, kf[2], kf[3]);
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[k_slot]);
     const int p0 = t * TILE + kw;
     const bool masked = t * TILE < e.start || (t + 1) * TILE > block_lo_hi;
     float top[2] = {-INFINITY, -INFINITY};
@@ -266,6 +261,7 @@ __global__ void __launch_bounds__(ROWS_THREADS)
         s[i][x] = exp2f(s[i][x] - (base[x >> 1] - P_SHIFT));
         l[x >> 1] += s[i][x];
       }
+    ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
     // A value that is no number, at a position that only some of the rows see: a product with a weight of
     // 0 would spread it to the others, so it is added to the rows that see it and cleared for the product.
     if (masked && block_lo_hi < block_hi) {
@@ -347,11 +343,8 @@ __global__ void __launch_bounds__(ROWS_THREADS)
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[stage]);
-    if (++stage == ST) {
-      stage = 0;
-      phase ^= 1u;
-    }
+    if (lane == 0) mbar_arrive(&empty[ring.slot]);
+    ring.next();
   }
   if (!ok && lane == 0) {
     *abort_flag = 1;
@@ -424,6 +417,7 @@ __global__ void __launch_bounds__(ROWS_THREADS)
       }
     }
   }
+  if (!pre) own_leave(a);
 }
 
 // Join the parts of each (token, head): a warp takes `heads` heads of a token, lane x elements 4 x ... and,
@@ -565,7 +559,7 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
     // short runs and no prefix: a block each, which needs no join; a tile takes a block about 0.5 us, a join 3
     const long long runs = static_cast<long long>(n_batch) * n_kv * ((rep + 15) / 16);
     if ((shared_len > 0 || own_tiles > 8) && runs * own_tiles <= INT_MAX)
-      p.own_ctas = static_cast<int>(std::min(static_cast<long long>(attn_one_blocks(hd, rep, n_batch)), runs * own_tiles));
+      p.own_ctas = static_cast<int>(std::min(static_cast<long long>(attn_one_blocks(hd, rep, n_batch, runs * own_tiles)), runs * own_tiles));
     else if (shared_len > 0)
       p.one = false;
   }
@@ -606,17 +600,17 @@ size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 size_t work_bytes(const AttnPlan& p, int n_batch, int n_tokens, int n_heads, int hd) {
   const size_t rows = static_cast<size_t>(part_rows(p, n_tokens, n_heads));
+  if (rows == 0) return 0;
   return up256(rows * 8) + up256(rows * hd * 4) + up256((static_cast<size_t>(n_batch) + 1) * 4);
 }
 
 template <typename T, int DP, int WM>
 cudaError_t launch_rows_as(const AttnArgs& a, uint32_t type, int blocks, int splits, int pre, cudaStream_t st) {
   using L = RowsLayout<DP, WM>;
-  static const cudaError_t set =
-      cudaFuncSetAttribute(attn_rows_kernel<T, DP, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
+  static const cudaError_t set = allow_smem(attn_rows_kernel<T, DP, WM>, L::ALLOC);
   if (set != cudaSuccess) return set;
   CUtensorMap kmap, vmap;
-  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type, TILE) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type, TILE))
+  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type))
     return cudaErrorInvalidValue;
   return launch_dependent(attn_rows_kernel<T, DP, WM>, dim3(blocks, a.c.n_kv, splits), dim3(ROWS_THREADS), L::ALLOC, st, a, kmap, vmap, pre);
 }
@@ -692,7 +686,7 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   const size_t need = ex::work_bytes(p, n_batch, n_tokens, n_heads, a.c.hd);
   const long long rows = static_cast<long long>(n_tokens) * n_heads;
   if (rows > INT_MAX || p.own_blocks < 0) return ex::api_fail(nullptr, 0, "kv_attention: %d tokens in one call", n_tokens);
-  if (work == nullptr || work_size < need || (reinterpret_cast<uintptr_t>(work) & 255) != 0)
+  if (need > 0 && (work == nullptr || work_size < need || (reinterpret_cast<uintptr_t>(work) & 255) != 0))
     return ex::api_fail(nullptr, 0, "kv_attention: work memory of %zu bytes, 256-byte aligned, is needed (got %zu)", need,
                         work == nullptr ? static_cast<size_t>(0) : work_size);
   a.layer_off = layer * a.c.layer_stride;
@@ -719,6 +713,7 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   a.cont_row0 = static_cast<long long>(p.n_pre + p.n_own) * rows;
   a.out = out;
   a.out_f32 = out_type == ex::TYPE_F32;
+  a.beside = p.n_pre > 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = cache->type == ex::TYPE_F16 ? ex::launch_attention_as<__half>(a, p, cache->type, st)
                                                     : ex::launch_attention_as<__nv_bfloat16>(a, p, cache->type, st);

@@ -34,7 +34,20 @@ struct AttnArgs {
   float2* part_ml;   // [n_pre + n_own][token][head]: m, l
   void* out;
   int out_f32;
+  int beside;        // the own pass runs beside the shared pass, launched before it
 };
+
+// The own pass' way in and out: beside a shared pass it starts at once, and the last of its blocks waits
+// for that pass, so that both are complete when it is.
+__device__ __forceinline__ void own_enter(const AttnArgs& a) {
+  if (a.beside)
+    pdl_launch_next();
+  else
+    pdl_enter_grid();
+}
+__device__ __forceinline__ void own_leave(const AttnArgs& a) {
+  if (a.beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) pdl_wait_previous();
+}
 
 // Positions of the prefix.
 __device__ __forceinline__ int shared_of(const AttnArgs& a) {
@@ -120,14 +133,67 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A layer of a pool as [page][head x slot][element], in boxes of 64 elements of at most `most` of a
-// page's positions; elements past head_dim read as 0 (kvattn_tc.cu).
-bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type, int most);
+// A layer of a pool as [page][head x slot][element], in boxes of 64 elements of at most 64 of a page's
+// positions; elements past head_dim read as 0 (kvattn_tc.cu).
+bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type);
 
 // Launch the single tokens' own pass (kvattn_one.cu), hd at most 128; its blocks where the line is cut.
 constexpr int ONE_MAX_BATCH = 2048;  // the runs' offsets are in shared memory
 cudaError_t launch_attn_one(const AttnArgs& a, uint32_t type, cudaStream_t st);
-int attn_one_blocks(int hd, int rep, int n_batch);
+int attn_one_blocks(int hd, int rep, int n_batch, long long tiles);
+
+// A place in a ring of slots, and the parity of its filling.
+template <int NS>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == NS) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  __device__ __forceinline__ void back() {
+    if (--slot < 0) {
+      slot = NS - 1;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Wait for the last fillings of a ring that has got `issued` of them (NS or fewer count), `ring` being the
+// place of the next: no copy may still be landing when a block exits.
+template <int NS>
+__device__ __forceinline__ void drain(const Ring<NS>& ring, int issued, uint64_t* full, uint32_t* status) {
+  bool drained = true;
+  for (int n = min(issued, NS); n > 0; --n) {
+    const int s = ring.slot - n + (ring.slot < n ? NS : 0);
+    if (!mbar_wait(&full[s], ring.phase ^ (ring.slot < n ? 1u : 0u))) drained = false;
+  }
+  if (!drained) atomicOr(status, ST_TIMEOUT_DRAIN);
+}
+
+// One warp: positions [p0, end) of head kvh, at most ROWS of them and from a multiple of ROWS, into a slot as
+// ROWS rows of 128 bytes for each 64 elements.  Boxes of rows: lane x brings the page of the x-th one.
+template <int DP, int ROWS>
+__device__ __forceinline__ void bring_tile(const KvView& c, const int32_t* table, const CUtensorMap* map, uint32_t dst, int kvh, int p0,
+                                           int end, uint64_t* bar) {
+  const int lane = threadIdx.x & 31, box = min(1 << c.ps_shift, TILE), boxes = (min(ROWS, end - p0) + box - 1) / box;
+  const int p = p0 + lane * box;
+  if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box * DP * 2);
+  __syncwarp();
+  if (lane < boxes) {
+    int page = table[p >> c.ps_shift];
+    if (page < 0 || page >= c.n_pages) {
+      atomicOr(c.status, ST_BAD_CACHE);
+      page = 0;
+    }
+    const int y = (kvh << c.ps_shift) + (p & ((1 << c.ps_shift) - 1));
+#pragma unroll
+    for (int h = 0; h < DP / 64; ++h) tma_3d(dst + lane * box * 128 + h * ROWS * 128, map, 64 * h, y, page, bar);
+  }
+  __syncwarp();
+}
 
 // Launch the shared pass on the tensor cores' own memory (kvattn_tc.cu), hd at most 128.
 cudaError_t launch_attn_tc(const AttnArgs& a, uint32_t type, cudaStream_t st);

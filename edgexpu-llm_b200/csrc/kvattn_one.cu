@@ -26,11 +26,11 @@ constexpr int ONE_THREADS = 160;
 
 template <int DP>
 struct OneLayout {
-  static constexpr int STAGES = DP == 64 ? 4 : 3;
+  static constexpr int SLOTS = DP == 64 ? 10 : 6;
   static constexpr int HALF = TILE * 128;
-  static constexpr int KV = HALF * (DP / 64);  // a tile of K, or of V
-  static constexpr int BARS = STAGES * 2 * KV;
-  static constexpr int FIXED = BARS + 8 * 2 * STAGES + 64;
+  static constexpr int SLOT = HALF * (DP / 64);  // a tile of K, or of V
+  static constexpr int BARS = SLOTS * SLOT;
+  static constexpr int FIXED = BARS + 8 * 2 * SLOTS + 64;
 };
 
 // Dynamic shared memory: ring, barriers, the four warps' sums for a run's join, the runs' offsets.
@@ -46,10 +46,10 @@ struct Run {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(ONE_THREADS)
+__global__ void __launch_bounds__(ONE_THREADS, 2)
     attn_one_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using L = OneLayout<DP>;
-  constexpr int ST = L::STAGES;
+  constexpr int ST = L::SLOTS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(ONE_THREADS)
     *quit = 0;
     fence_mbar_init();
   }
-  pdl_enter_grid();
+  own_enter(a);
   const int shared = shared_of(a);
   const int per_entry = a.c.n_kv * n_rb;  // runs of an entry
   const bool whole = a.own_ctas == 0;
@@ -159,42 +159,20 @@ __global__ void __launch_bounds__(ONE_THREADS)
   const long long stop = whole ? 1 : end;
 
   if (warp == 4) {
-    const int box = min(1 << a.c.ps_shift, TILE);
-    int stage = 0, issued = 0, i = first_entry;
-    uint32_t phase = 0;
+    Ring<ST> ring;
+    int issued = 0, i = first_entry;
     bool ok = true;
     for (long long at = begin; ok && at < stop;) {
       const Run r = run_at(at, i);
       at += whole ? 1 : r.n;
       const int32_t* table = a.c.table + static_cast<long long>(max(0, r.row)) * a.c.max_pages;
-      for (int t = r.tile0; t < r.tile0 + r.n; ++t) {
-        const int p = t * TILE + lane * box, boxes = (min(TILE, r.len - t * TILE) + box - 1) / box;
-        int page = 0;
-        if (lane < boxes) {
-          page = table[p >> a.c.ps_shift];
-          if (page < 0 || page >= a.c.n_pages) {
-            atomicOr(a.c.status, ST_BAD_CACHE);
-            page = 0;
-          }
-        }
-        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[stage], phase ^ 1u, abort_flag));
+      for (int t = 2 * r.tile0; ok && t < 2 * (r.tile0 + r.n); ++t) {  // K of a tile, then its V
+        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
         if (!ok) break;
+        bring_tile<DP, TILE>(a.c, table, (t & 1) == 0 ? &kmap : &vmap, smem_u32(smem + ring.slot * L::SLOT), r.kvh, (t >> 1) * TILE, r.len,
+                       &full[ring.slot]);
         issued = min(issued + 1, ST);
-        if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box * DP * 4);
-        __syncwarp();
-        if (lane < boxes) {
-          const uint32_t dst = smem_u32(smem + stage * 2 * L::KV) + lane * box * 128;
-          const int y = (r.kvh << a.c.ps_shift) + (p & ((1 << a.c.ps_shift) - 1));
-#pragma unroll
-          for (int h = 0; h < DP / 64; ++h) {
-            tma_3d(dst + h * L::HALF, &kmap, 64 * h, y, page, &full[stage]);
-            tma_3d(dst + L::KV + h * L::HALF, &vmap, 64 * h, y, page, &full[stage]);
-          }
-        }
-        if (++stage == ST) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        ring.next();
       }
     }
     if (lane == 0) {
@@ -202,17 +180,12 @@ __global__ void __launch_bounds__(ONE_THREADS)
         *abort_flag = 1;
         atomicOr(a.c.status, ST_TIMEOUT_EMPTY);
       }
-      bool drained = true;  // no copy may still be landing when the block exits
-      for (int n = issued; n > 0; --n) {
-        const int s = stage - n + (stage < n ? ST : 0);
-        if (!mbar_wait(&full[s], phase ^ (stage < n ? 1u : 0u))) drained = false;
-      }
-      if (!drained) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
+      drain<ST>(ring, issued, full, a.c.status);
     }
   } else {
     const int g = lane >> 3, lr = lane & 7, kw = warp * 16, hd = a.c.hd;
-    int stage = 0, i = first_entry;
-    uint32_t phase = 0;
+    Ring<ST> ring;
+    int i = first_entry;
     bool ok = true;
     for (long long at = begin; ok && at < stop;) {
       const Run r = run_at(at, i);
@@ -232,12 +205,16 @@ __global__ void __launch_bounds__(ONE_THREADS)
       for (int x = 0; x < DP / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.0f;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
       for (int t = r.tile0; t < r.tile0 + r.n; ++t) {
-        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[stage], phase, abort_flag));
+        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
         if (!ok) break;
-        const uint32_t ks = smem_u32(smem + stage * 2 * L::KV), vs = ks + L::KV;
+        const uint32_t ks = smem_u32(smem + ring.slot * L::SLOT);
+        const Ring<ST> k = ring;
+        ring.next();
+        const uint32_t vs = smem_u32(smem + ring.slot * L::SLOT);
         const int p0 = t * TILE + kw;
-        if (p0 < r.len && p0 + 16 > r.start) {
-          float s[2][4] = {};
+        const bool in = p0 < r.len && p0 + 16 > r.start;
+        float s[2][4] = {};
+        if (in) {
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             uint32_t kf[4];
@@ -246,6 +223,12 @@ __global__ void __launch_bounds__(ONE_THREADS)
             mma16816<T>(s[0], q[kk], kf[0], kf[1]);
             mma16816<T>(s[1], q[kk], kf[2], kf[3]);
           }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[k.slot]);
+        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
+        if (!ok) break;
+        if (in) {
           const bool edge = p0 < r.start || p0 + 16 > r.len;  // some of the 16 positions are not the run's
           uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
           float top[2] = {-INFINITY, -INFINITY};
@@ -311,11 +294,8 @@ __global__ void __launch_bounds__(ONE_THREADS)
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[stage]);
-        if (++stage == ST) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (lane == 0) mbar_arrive(&empty[ring.slot]);
+        ring.next();
       }
       // join the four warps' positions; all of them get here, a given-up wait included
       if (!ok && lane == 0) {
@@ -372,22 +352,24 @@ __global__ void __launch_bounds__(ONE_THREADS)
       named_bar_sync(1, 128);  // before the next run's sums
     }
   }
+  own_leave(a);
 }
 
+// One round of blocks, or two where they get at least 16 tiles each: SMs do not get the same share of a busy
+// memory, and the second round evens that out (128 sequences of 33 to 2000 positions: 185 -> 182 us).
 template <int DP>
-int blocks_of(int rep, int n_batch) {
+int blocks_of(int rep, int n_batch, long long tiles) {
   const size_t smem = one_smem<DP>(std::min(16, rep), n_batch, false);
-  const int fit = static_cast<int>((228 * 1024) / (smem + 1024));
-  return std::max(1, std::min(fit, 4)) * api_device_info().sm_count;
+  const int round = std::max(1, std::min(static_cast<int>((228 * 1024) / (smem + 1024)), 2)) * api_device_info().sm_count;
+  return tiles >= 32LL * round ? 2 * round : round;
 }
 
 template <typename T, int DP>
 cudaError_t launch_one_as(const AttnArgs& a, uint32_t type, int blocks, cudaStream_t st) {
-  static const cudaError_t set =
-      cudaFuncSetAttribute(attn_one_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  static const cudaError_t set = allow_smem(attn_one_kernel<T, DP>, 200 * 1024);
   if (set != cudaSuccess) return set;
   CUtensorMap kmap, vmap;
-  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type, TILE) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type, TILE))
+  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type))
     return cudaErrorInvalidValue;
   return launch_dependent(attn_one_kernel<T, DP>, dim3(blocks), dim3(ONE_THREADS),
                           one_smem<DP>(std::min(16, a.rep), a.n_batch, a.own_ctas == 0), st, a, kmap, vmap);
@@ -395,7 +377,9 @@ cudaError_t launch_one_as(const AttnArgs& a, uint32_t type, int blocks, cudaStre
 
 }  // namespace
 
-int attn_one_blocks(int hd, int rep, int n_batch) { return hd <= 64 ? blocks_of<64>(rep, n_batch) : blocks_of<128>(rep, n_batch); }
+int attn_one_blocks(int hd, int rep, int n_batch, long long tiles) {
+  return hd <= 64 ? blocks_of<64>(rep, n_batch, tiles) : blocks_of<128>(rep, n_batch, tiles);
+}
 
 cudaError_t launch_attn_one(const AttnArgs& a, uint32_t type, cudaStream_t st) {
   const int blocks = a.own_ctas > 0 ? a.own_ctas : a.n_batch * a.c.n_kv * ((a.rep + 15) / 16);

@@ -127,10 +127,10 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// The larger; NaN if either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
+// The largest; NaN if any is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -146,27 +146,8 @@ __device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
-// A place in the ring of slots, and the parity of its filling.
-template <int NS>
-struct Ring {
-  int slot = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == NS) {
-      slot = 0;
-      phase ^= 1u;
-    }
-  }
-  __device__ __forceinline__ void back() {
-    if (--slot < 0) {
-      slot = NS - 1;
-      phase ^= 1u;
-    }
-  }
-};
-
 // A block of rows along consecutive tiles of the prefix, in steps of half a tile.
-constexpr int STEP = TC_TILE / 2;
+constexpr int STEP = TILE;
 struct Segment {
   int kvh, row0, tile0, n, slot;
   int steps;  // the prefix's last half tile may be empty
@@ -234,7 +215,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   __syncthreads();
   tc_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
-  pdl_enter_grid();
+  pdl_enter_pair();
 
   const int shared = __shfl_sync(0xFFFFFFFFu, shared_of(a), 0);
   const TcCut cut = tc_cut(a, shared);
@@ -242,40 +223,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   if (warp == 0) {
     // K of tile 0, V of tile 0, K of tile 1, ...: the order in which the products need them
-    const int box = min(1 << a.c.ps_shift, TC_TILE);  // positions a box holds
     const int32_t* table = a.c.table + static_cast<long long>(a.shared_seq) * a.c.max_pages;
     Ring<NS> ring;
-    int issued = 0;  // slots filled, NS at most
+    int issued = 0;
     bool ok = true;
     for (int at = begin; ok && at < end;) {
       const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
       at += g.n;
-      for (int i = 0; ok && i < g.n; ++i) {
-        const int p0 = (g.tile0 + i) * TC_TILE;
-        const int boxes = (min(TC_TILE, shared - p0) + box - 1) / box;
-        int page = 0;
-        const int p = p0 + lane * box;
-        if (lane < boxes) {
-          page = table[p >> a.c.ps_shift];
-          if (page < 0 || page >= a.c.n_pages) {
-            atomicOr(a.c.status, ST_BAD_CACHE);
-            page = 0;
-          }
-        }
-        for (int kv = 0; kv < 2; ++kv, ring.next()) {
-          const int slot = ring.slot;
-          ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[slot], ring.phase ^ 1u, abort_flag));
-          if (!ok) break;
-          issued = min(issued + 1, NS);
-          if (lane == 0) mbar_arrive_expect_tx(&full[slot], boxes * box * DP * 2);
-          __syncwarp();
-          if (lane < boxes) {
-            const uint32_t dst = smem_u32(smem + L::RING + slot * L::SLOT) + lane * box * 128;
-            const int y = (g.kvh << a.c.ps_shift) + (p & ((1 << a.c.ps_shift) - 1));
-#pragma unroll
-            for (int h = 0; h < DP / 64; ++h) tma_3d(dst + h * L::HALF, kv == 0 ? &kmap : &vmap, 64 * h, y, page, &full[slot]);
-          }
-        }
+      for (int i = 0; ok && i < 2 * g.n; ++i) {
+        ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
+        if (!ok) break;
+        bring_tile<DP, TC_TILE>(a.c, table, (i & 1) == 0 ? &kmap : &vmap, smem_u32(smem + L::RING + ring.slot * L::SLOT), g.kvh,
+                                (g.tile0 + (i >> 1)) * TC_TILE, shared, &full[ring.slot]);
+        issued = min(issued + 1, NS);
+        ring.next();
       }
     }
     if (lane == 0) {
@@ -283,13 +244,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         *abort_flag = 1;
         atomicOr(a.c.status, ST_TIMEOUT_EMPTY);
       }
-      bool drained = true;  // no copy may still be landing when the block exits
-      for (int n = 0; n < issued; ++n) {  // the last filling of each slot, from the oldest
-        const int back = issued - n;
-        const int slot = ring.slot - back + (ring.slot < back ? NS : 0);
-        if (!mbar_wait(&full[slot], ring.phase ^ (ring.slot < back ? 1u : 0u))) drained = false;
-      }
-      if (!drained) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
+      drain<NS>(ring, issued, full, a.c.status);
     }
   } else if (warp == 1) {
     // The warp runs the loop together and one thread issues: descriptors are then uniform where they are made.
@@ -456,10 +411,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         float top[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) top[c] = __uint_as_float(s[c]);
+        for (int c = 0; c < 4; ++c) top[c] = max_nan(__uint_as_float(s[3 * c]), __uint_as_float(s[3 * c + 1]), __uint_as_float(s[3 * c + 2]));
 #pragma unroll
-        for (int c = 4; c < STEP; ++c) top[c & 3] = max_nan(top[c & 3], __uint_as_float(s[c]));
-        const float tm = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * sc;
+        for (int c = 12; c < STEP; c += 2) top[(c >> 1) & 3] = max_nan(top[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        const float tm = max_nan(max_nan(top[0], top[1], top[2]), top[3], top[3]) * sc;
         if (j == 0) {
           m = tm;
         } else {
@@ -583,13 +538,13 @@ EncodeTiledFn kv_encode_tiled() {
 
 }  // namespace
 
-bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type, int most) {
+bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type) {
   EncodeTiledFn enc = kv_encode_tiled();
   if (enc == nullptr) return false;
   const int ps = 1 << c.ps_shift;
   const cuuint64_t dims[3] = {(cuuint64_t)c.hd, (cuuint64_t)c.n_kv * ps, (cuuint64_t)c.n_pages};
   const cuuint64_t strides[2] = {(cuuint64_t)c.hd * 2, (cuuint64_t)c.page_stride * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)(ps < most ? ps : most), 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(ps < TILE ? ps : TILE), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   return enc(map, type == TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
              const_cast<uint16_t*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -601,10 +556,10 @@ namespace {
 template <typename T, int DP, int MT>
 cudaError_t launch_tc_as(const AttnArgs& a, uint32_t type, cudaStream_t st) {
   using L = TcLayout<DP, MT>;
-  static const cudaError_t set = cudaFuncSetAttribute(attn_tc_kernel<T, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
+  static const cudaError_t set = allow_smem(attn_tc_kernel<T, DP, MT>, L::ALLOC);
   if (set != cudaSuccess) return set;
   CUtensorMap kmap, vmap;
-  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type, TC_TILE) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type, TC_TILE)) return cudaErrorInvalidValue;
+  if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type)) return cudaErrorInvalidValue;
   return launch_dependent(attn_tc_kernel<T, DP, MT>, dim3(a.pre_ctas), dim3(TC_THREADS), L::ALLOC, st, a, kmap, vmap);
 }
 

@@ -395,7 +395,7 @@ int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache *cache, int layer,
  * EDGEXPU_CUDA_TYPE_F32 (the next linear's input).  Products are of the cache's type (the softmax weights
  * are rounded to it), sums are fp32.  max_len bounds the sequences' lengths for the division of the work
  * only.  work: edgexpu_cuda_kv_attention_work_bytes bytes of device memory, 256-byte aligned, of this call's own until it
- * is done; the size depends on these numbers alone. */
+ * is done; the size depends on these numbers alone and may be 0. */
 int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache *cache, int layer, const void *q, const int32_t *seqs,
                                   const int32_t *q_start, int n_batch, int n_tokens, int n_heads, int shared_seq,
                                   int shared_len, int max_len, float scale, void *out, uint32_t out_type, void *work,
