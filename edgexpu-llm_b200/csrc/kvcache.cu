@@ -394,7 +394,7 @@ struct QkArgs {
   long long qs, ks, vs;
   int n_tokens, n_heads, layer;
   const float *qw, *kw;
-  float eps;
+  float eps, inv_hd;
   const float* rope;
   int rope_positions, rot, halves;
   const int32_t *seqs, *pos;
@@ -422,22 +422,23 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvVie
   constexpr int GROUPS = 32 / GS;
   extern __shared__ __align__(16) float rows[];  // [warp][group][QK_HEADS][GS * V * 4], for the last form only
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, gl = lane % GS, gr = lane / GS;
-  const long long unit = static_cast<long long>(blockIdx.x) * QK_WARPS + w;
-  const int t = static_cast<int>(unit / units);
-  if (t >= a.n_tokens) return;
-  const int per_token = a.n_heads + 2 * c.n_kv, nv = c.hd / 4;
-  const int h0 = (static_cast<int>(unit % units) * GROUPS + gr) * QK_HEADS;
+  const unsigned unit = blockIdx.x * QK_WARPS + w, t = unit / static_cast<unsigned>(units);
+  if (t >= static_cast<unsigned>(a.n_tokens)) return;
+  const int n_qk = a.n_heads + c.n_kv, per_token = n_qk + c.n_kv, nv = c.hd / 4;
+  const int h0 = (static_cast<int>(unit - t * units) * GROUPS + gr) * QK_HEADS;
+  // where head h of the token would begin, were all heads of its kind
+  const float* q = a.q + t * a.qs;
+  const float* k = a.k + t * a.ks - a.n_heads * c.hd;
+  const float* v = a.v + t * a.vs - n_qk * c.hd;
   float4 e[QK_HEADS][V];
+  float rms[QK_HEADS];
 #pragma unroll
   for (int i = 0; i < QK_HEADS; ++i) {
     const int h = h0 + i;
-    const float* x = h < a.n_heads           ? a.q + t * a.qs + static_cast<long long>(h) * c.hd
-                     : h < a.n_heads + c.n_kv ? a.k + t * a.ks + static_cast<long long>(h - a.n_heads) * c.hd
-                                              : a.v + t * a.vs + static_cast<long long>(h - a.n_heads - c.n_kv) * c.hd;
+    const float4* x = reinterpret_cast<const float4*>((h < a.n_heads ? q : h < n_qk ? k : v) + h * c.hd) + gl;
 #pragma unroll
     for (int u = 0; u < V; ++u)
-      e[i][u] = h < per_token && gl + u * GS < nv ? __ldcs(reinterpret_cast<const float4*>(x) + gl + u * GS)
-                                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      e[i][u] = h < per_token && gl + u * GS < nv ? __ldcs(x + u * GS) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   const int s = a.seqs[t], p = a.pos[t];
   bool live = s >= 0 && p >= 0;
@@ -453,28 +454,41 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvVie
   const float* cs = a.rope != nullptr && live ? a.rope + static_cast<long long>(p) * a.rot : nullptr;
   const int half = a.rot / 2;
 
-  // 1 / rms of each head, and the norm's weights
+  // 1 / rms of each head, and the norm's weights; a group of heads may hold queries and keys
 #pragma unroll
-  for (int i = 0; i < QK_HEADS; ++i) {
-    const int h = h0 + i;
-    const float* wt = h < a.n_heads ? a.qw : h < a.n_heads + c.n_kv ? a.kw : nullptr;
-    float ss = 0.0f;
+  for (int u = 0; u < V; ++u) {
+    const float4 one = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    const bool in = gl + u * GS < nv;
+    const float4 gq = in && a.qw != nullptr && h0 < a.n_heads ? reinterpret_cast<const float4*>(a.qw)[gl + u * GS] : one;
+    const float4 gk = in && a.kw != nullptr && h0 + QK_HEADS > a.n_heads ? reinterpret_cast<const float4*>(a.kw)[gl + u * GS] : one;
+    if (u == 0) {
 #pragma unroll
-    for (int u = 0; u < V; ++u) ss += e[i][u].x * e[i][u].x + e[i][u].y * e[i][u].y + e[i][u].z * e[i][u].z + e[i][u].w * e[i][u].w;
+      for (int i = 0; i < QK_HEADS; ++i) {
+        float ss = 0.0f;
 #pragma unroll
-    for (int o = GS / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    if (wt != nullptr) {
-      const float r = 1.0f / sqrtf(ss / static_cast<float>(c.hd) + a.eps);
+        for (int x = 0; x < V; ++x) ss += e[i][x].x * e[i][x].x + e[i][x].y * e[i][x].y + e[i][x].z * e[i][x].z + e[i][x].w * e[i][x].w;
+        rms[i] = ss;
+      }
 #pragma unroll
-      for (int u = 0; u < V; ++u) {
-        const int j = gl + u * GS;
-        if (j < nv) {
-          const float4 g = reinterpret_cast<const float4*>(wt)[j];
-          e[i][u].x = e[i][u].x * r * g.x;
-          e[i][u].y = e[i][u].y * r * g.y;
-          e[i][u].z = e[i][u].z * r * g.z;
-          e[i][u].w = e[i][u].w * r * g.w;
-        }
+      for (int o = GS / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < QK_HEADS; ++i) rms[i] += __shfl_xor_sync(0xFFFFFFFFu, rms[i], o);
+#pragma unroll
+      for (int i = 0; i < QK_HEADS; ++i) {
+        const int h = h0 + i;
+        const bool normed = h < a.n_heads ? a.qw != nullptr : h < n_qk && a.kw != nullptr;
+        rms[i] = normed ? rsqrtf(rms[i] * a.inv_hd + a.eps) : 1.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < QK_HEADS; ++i) {
+      const int h = h0 + i;
+      if (h < n_qk) {
+        const float4 g = h < a.n_heads ? gq : gk;
+        e[i][u].x = e[i][u].x * rms[i] * g.x;
+        e[i][u].y = e[i][u].y * rms[i] * g.y;
+        e[i][u].z = e[i][u].z * rms[i] * g.z;
+        e[i][u].w = e[i][u].w * rms[i] * g.w;
       }
     }
   }
@@ -542,23 +556,21 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvVie
       for (int u = 0; u < V; ++u) e[i][u] = reinterpret_cast<float4*>(row + i * GS * V * 4)[gl + u * GS];
   }
 
+  // the same for where they go; pools are spaced by pages
+  uint16_t* q_to = a.q_out + static_cast<long long>(t) * a.n_heads * c.hd;
+  const long long slot = a.layer * c.layer_stride + page * c.page_stride + (p & ((1 << c.ps_shift) - 1)) * c.hd;
+  const int page_head = c.hd << c.ps_shift;
+  uint16_t* k_to = c.k + slot - static_cast<long long>(a.n_heads) * page_head;
+  uint16_t* v_to = c.v + slot - static_cast<long long>(n_qk) * page_head;
 #pragma unroll
   for (int i = 0; i < QK_HEADS; ++i) {
     const int h = h0 + i;
-    if (h >= per_token) break;
-    uint16_t* dst = a.q_out + (static_cast<long long>(t) * a.n_heads + h) * c.hd;
-    if (h >= a.n_heads) {
-      if (!live) break;
-      const bool is_k = h < a.n_heads + c.n_kv;
-      const int hh = is_k ? h - a.n_heads : h - a.n_heads - c.n_kv;
-      dst = (is_k ? c.k : c.v) + a.layer * c.layer_stride + page * c.page_stride +
-            ((static_cast<long long>(hh) << c.ps_shift) + (p & ((1 << c.ps_shift) - 1))) * c.hd;
-    }
+    if (h >= per_token || (h >= a.n_heads && !live)) break;
+    uint2* to = reinterpret_cast<uint2*>(h < a.n_heads ? q_to + h * c.hd : (h < n_qk ? k_to : v_to) + static_cast<long long>(h) * page_head) + gl;
 #pragma unroll
     for (int u = 0; u < V; ++u)
       if (gl + u * GS < nv)
-        reinterpret_cast<uint2*>(dst)[gl + u * GS] =
-            live ? make_uint2(pack16<T>(e[i][u].x, e[i][u].y), pack16<T>(e[i][u].z, e[i][u].w)) : make_uint2(0u, 0u);
+        to[u * GS] = live ? make_uint2(pack16<T>(e[i][u].x, e[i][u].y), pack16<T>(e[i][u].z, e[i][u].w)) : make_uint2(0u, 0u);
   }
 }
 
@@ -567,7 +579,7 @@ cudaError_t launch_heads_as(const KvView& c, QkArgs a, cudaStream_t st) {
   const int at_once = QK_HEADS * (32 / GS);
   const int units = (a.n_heads + 2 * c.n_kv + at_once - 1) / at_once;
   const long long blocks = (static_cast<long long>(a.n_tokens) * units + QK_WARPS - 1) / QK_WARPS;
-  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  if (blocks > INT_MAX / QK_WARPS) return cudaErrorInvalidValue;  // units are counted in 32 bits
   if (a.rope == nullptr)
     a.form = QkArgs::NONE;
   else if (!a.halves)
@@ -723,7 +735,7 @@ int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   if (rope_pairing != EDGEXPU_CUDA_ROPE_ADJACENT && rope_pairing != EDGEXPU_CUDA_ROPE_HALVES)
     return ex::api_fail(nullptr, 0, "qk_norm_rope: pairing %d", rope_pairing);
   if (n_tokens == 0) return 1;
-  const ex::QkArgs a{q, k, v, q_stride, k_stride, v_stride, n_tokens, n_heads, layer, q_weight, k_weight, eps, rope,
+  const ex::QkArgs a{q, k, v, q_stride, k_stride, v_stride, n_tokens, n_heads, layer, q_weight, k_weight, eps, 1.0f / static_cast<float>(c.hd), rope,
                      rope_positions, rope_dims, rope_pairing == EDGEXPU_CUDA_ROPE_HALVES, seqs, pos,
                      static_cast<uint16_t*>(q_out), ex::QkArgs::NONE};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
