@@ -399,7 +399,6 @@ struct QkArgs {
   int rope_positions, rot, halves;
   const int32_t *seqs, *pos;
   uint16_t* q_out;
-  enum { NONE, IN_LANE, BETWEEN_LANES, IN_SHARED } form;  // where a pair is turned
 };
 
 constexpr int QK_WARPS = 8;
@@ -412,119 +411,108 @@ __device__ __forceinline__ void rotate(float& y0, float& y1, float c, float s) {
   y0 = a;
 }
 
-// A group of GS lanes takes QK_HEADS heads of a token, a lane V times four elements of each: the
-// token's page and angles are looked up once for them, the sums of squares are fp32 over the group, and
-// a pair is turned in its lane (adjacent), between two lanes (halves, in whole chunks of four) or, for
-// the other splits of a head, in shared memory.  Bound by HBM (4 bytes read and 2 written an element).
-template <typename T, int GS, int V>
+// Where the pairs of a head are turned: nowhere, in the lane that holds both (adjacent), between two lanes
+// (halves, in whole chunks of four elements), or in shared memory (the other splits of a head).
+enum class Turn { None, InLane, BetweenLanes, InShared };
+
+// A group of GS lanes takes QK_HEADS heads of a token, all queries, all keys or all values, a lane V times
+// four elements of each: the token's page, angles and weights are looked up once for them, and the sums of
+// squares are fp32 over the group.  Bytes are 4 read and 2 written an element; at 8k tokens of 48 heads of
+// 128 it is bound by the instructions it issues, about 110 a head and warp.
+template <typename T, int GS, int V, Turn TURN>
 __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvView c, const QkArgs a, const int units) {
   pdl_enter_grid();
   constexpr int GROUPS = 32 / GS;
-  extern __shared__ __align__(16) float rows[];  // [warp][group][QK_HEADS][GS * V * 4], for the last form only
+  extern __shared__ __align__(16) float rows[];  // [warp][group][QK_HEADS][GS * V * 4], for Turn::InShared
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, gl = lane % GS, gr = lane / GS;
   const unsigned unit = blockIdx.x * QK_WARPS + w, t = unit / static_cast<unsigned>(units);
   if (t >= static_cast<unsigned>(a.n_tokens)) return;
-  const int n_qk = a.n_heads + c.n_kv, per_token = n_qk + c.n_kv, nv = c.hd / 4;
-  const int h0 = (static_cast<int>(unit - t * units) * GROUPS + gr) * QK_HEADS;
-  // where head h of the token would begin, were all heads of its kind
-  const float* q = a.q + t * a.qs;
-  const float* k = a.k + t * a.ks - a.n_heads * c.hd;
-  const float* v = a.v + t * a.vs - n_qk * c.hd;
+  const int nv = c.hd / 4, q_groups = (a.n_heads + QK_HEADS - 1) / QK_HEADS, k_groups = (c.n_kv + QK_HEADS - 1) / QK_HEADS;
+  int group = static_cast<int>(unit - t * units) * GROUPS + gr;
+  const bool is_q = group < q_groups, is_k = !is_q && group < q_groups + k_groups;
+  const float* x = is_q ? a.q + t * a.qs : is_k ? a.k + t * a.ks : a.v + t * a.vs;
+  const float* wt = is_q ? a.qw : is_k ? a.kw : nullptr;
+  const int h0 = (is_q ? group : is_k ? group - q_groups : group - q_groups - k_groups) * QK_HEADS;
+  const int n = min(QK_HEADS, (is_q ? a.n_heads : c.n_kv) - h0);  // heads of the group, none in a last one past the values
   float4 e[QK_HEADS][V];
-  float rms[QK_HEADS];
+  const float4* x4 = reinterpret_cast<const float4*>(x + h0 * c.hd) + gl;
 #pragma unroll
-  for (int i = 0; i < QK_HEADS; ++i) {
-    const int h = h0 + i;
-    const float4* x = reinterpret_cast<const float4*>((h < a.n_heads ? q : h < n_qk ? k : v) + h * c.hd) + gl;
+  for (int i = 0; i < QK_HEADS; ++i)
 #pragma unroll
-    for (int u = 0; u < V; ++u)
-      e[i][u] = h < per_token && gl + u * GS < nv ? __ldcs(x + u * GS) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
+    for (int u = 0; u < V; ++u) e[i][u] = i < n && gl + u * GS < nv ? __ldcs(x4 + i * nv + u * GS) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int s = a.seqs[t], p = a.pos[t];
   bool live = s >= 0 && p >= 0;
   int page = -1;
   if (live) {
-    if (s < c.n_seqs && (p >> c.ps_shift) < c.max_pages && (a.rope == nullptr || p < a.rope_positions))
+    if (s < c.n_seqs && (p >> c.ps_shift) < c.max_pages && (TURN == Turn::None || p < a.rope_positions))
       page = c.table[static_cast<long long>(s) * c.max_pages + (p >> c.ps_shift)];
     if (page < 0 || page >= c.n_pages) {
       live = false;
       if (lane == 0) atomicOr(c.status, ST_BAD_CACHE);
     }
   }
-  const float* cs = a.rope != nullptr && live ? a.rope + static_cast<long long>(p) * a.rot : nullptr;
-  const int half = a.rot / 2;
-
-  // 1 / rms of each head, and the norm's weights; a group of heads may hold queries and keys
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
-    const float4 one = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-    const bool in = gl + u * GS < nv;
-    const float4 gq = in && a.qw != nullptr && h0 < a.n_heads ? reinterpret_cast<const float4*>(a.qw)[gl + u * GS] : one;
-    const float4 gk = in && a.kw != nullptr && h0 + QK_HEADS > a.n_heads ? reinterpret_cast<const float4*>(a.kw)[gl + u * GS] : one;
-    if (u == 0) {
-#pragma unroll
-      for (int i = 0; i < QK_HEADS; ++i) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int x = 0; x < V; ++x) ss += e[i][x].x * e[i][x].x + e[i][x].y * e[i][x].y + e[i][x].z * e[i][x].z + e[i][x].w * e[i][x].w;
-        rms[i] = ss;
-      }
-#pragma unroll
-      for (int o = GS / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < QK_HEADS; ++i) rms[i] += __shfl_xor_sync(0xFFFFFFFFu, rms[i], o);
-#pragma unroll
-      for (int i = 0; i < QK_HEADS; ++i) {
-        const int h = h0 + i;
-        const bool normed = h < a.n_heads ? a.qw != nullptr : h < n_qk && a.kw != nullptr;
-        rms[i] = normed ? rsqrtf(rms[i] * a.inv_hd + a.eps) : 1.0f;
-      }
-    }
+  if (wt != nullptr || GROUPS > 1) {  // 1 / rms of each head, and the norm's weights
+    float rms[QK_HEADS];
 #pragma unroll
     for (int i = 0; i < QK_HEADS; ++i) {
-      const int h = h0 + i;
-      if (h < n_qk) {
-        const float4 g = h < a.n_heads ? gq : gk;
-        e[i][u].x = e[i][u].x * rms[i] * g.x;
-        e[i][u].y = e[i][u].y * rms[i] * g.y;
-        e[i][u].z = e[i][u].z * rms[i] * g.z;
-        e[i][u].w = e[i][u].w * rms[i] * g.w;
+      rms[i] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < V; ++u) rms[i] += e[i][u].x * e[i][u].x + e[i][u].y * e[i][u].y + e[i][u].z * e[i][u].z + e[i][u].w * e[i][u].w;
+    }
+#pragma unroll
+    for (int o = GS / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < QK_HEADS; ++i) rms[i] += __shfl_xor_sync(0xFFFFFFFFu, rms[i], o);
+    if (wt != nullptr) {
+#pragma unroll
+      for (int i = 0; i < QK_HEADS; ++i) rms[i] = rsqrtf(rms[i] * a.inv_hd + a.eps);
+#pragma unroll
+      for (int u = 0; u < V; ++u) {
+        const float4 g = gl + u * GS < nv ? reinterpret_cast<const float4*>(wt)[gl + u * GS] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < QK_HEADS; ++i) {
+          e[i][u].x = e[i][u].x * rms[i] * g.x;
+          e[i][u].y = e[i][u].y * rms[i] * g.y;
+          e[i][u].z = e[i][u].z * rms[i] * g.z;
+          e[i][u].w = e[i][u].w * rms[i] * g.w;
+        }
       }
     }
   }
 
-  const int turned = min(QK_HEADS, a.n_heads + c.n_kv - h0);  // q and k heads of the group, may be none
-  if (a.form == QkArgs::IN_LANE) {
+  const bool turned = live && (is_q || is_k);
+  const float* cs = turned ? a.rope + static_cast<long long>(p) * a.rot : a.rope;
+  const int half = a.rot / 2;
+  if constexpr (TURN == Turn::InLane) {
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const int j = gl + u * GS;
-      if (cs != nullptr && 4 * j < a.rot) {
-        const float2 a0 = *reinterpret_cast<const float2*>(cs + 4 * j);
+      if (turned && 4 * j < a.rot) {
         const bool both = 4 * j + 2 < a.rot;
+        const float2 a0 = *reinterpret_cast<const float2*>(cs + 4 * j);
         const float2 a1 = both ? *reinterpret_cast<const float2*>(cs + 4 * j + 2) : make_float2(1.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < QK_HEADS; ++i)
-          if (i < turned) {
-            rotate(e[i][u].x, e[i][u].y, a0.x, a0.y);
-            if (both) rotate(e[i][u].z, e[i][u].w, a1.x, a1.y);
-          }
+        for (int i = 0; i < QK_HEADS; ++i) rotate(e[i][u].x, e[i][u].y, a0.x, a0.y);
+        if (both)
+#pragma unroll
+          for (int i = 0; i < QK_HEADS; ++i) rotate(e[i][u].z, e[i][u].w, a1.x, a1.y);
       }
     }
-  } else if (a.form == QkArgs::BETWEEN_LANES) {
+  } else if constexpr (TURN == Turn::BetweenLanes) {
     // V == 1 and half % 4 == 0: chunk j < half / 4 turns with chunk j + half / 4, half / 4 lanes on
     const int step = half / 4;
-    const bool low = gl < step, in = gl < 2 * step;
+    const bool low = gl < step, in = turned && gl < 2 * step;
     float ang[8] = {1.0f, 0.0f, 1.0f, 0.0f, 1.0f, 0.0f, 1.0f, 0.0f};
-    if (cs != nullptr && in) {
+    if (in) {
       const float2* at = reinterpret_cast<const float2*>(cs) + 4 * (low ? gl : gl - step);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 x = at[k];
-        ang[2 * k] = x.x;
-        ang[2 * k + 1] = low ? -x.y : x.y;  // y0 c - y1 s below, y1 c + y0 s above
+        const float2 y = at[k];
+        ang[2 * k] = y.x;
+        ang[2 * k + 1] = low ? -y.y : y.y;  // y0 c - y1 s below, y1 c + y0 s above
       }
     }
-    const int from = gr * GS + (low ? gl + step : in ? gl - step : gl);
+    const int from = gr * GS + (low ? gl + step : gl < 2 * step ? gl - step : gl);
 #pragma unroll
     for (int i = 0; i < QK_HEADS; ++i) {
       const float4 mine = e[i][0];
@@ -533,22 +521,22 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvVie
       other.y = __shfl_sync(0xFFFFFFFFu, mine.y, from);
       other.z = __shfl_sync(0xFFFFFFFFu, mine.z, from);
       other.w = __shfl_sync(0xFFFFFFFFu, mine.w, from);
-      if (i < turned && in && cs != nullptr) {
+      if (in) {
         e[i][0].x = mine.x * ang[0] + other.x * ang[1];
         e[i][0].y = mine.y * ang[2] + other.y * ang[3];
         e[i][0].z = mine.z * ang[4] + other.z * ang[5];
         e[i][0].w = mine.w * ang[6] + other.w * ang[7];
       }
     }
-  } else if (a.form == QkArgs::IN_SHARED) {
+  } else if constexpr (TURN == Turn::InShared) {
     float* row = rows + (w * GROUPS + gr) * QK_HEADS * GS * V * 4;
 #pragma unroll
     for (int i = 0; i < QK_HEADS; ++i)
 #pragma unroll
       for (int u = 0; u < V; ++u) reinterpret_cast<float4*>(row + i * GS * V * 4)[gl + u * GS] = e[i][u];
     __syncwarp();
-    for (int j = gl; j < half && cs != nullptr; j += GS)
-      for (int i = 0; i < turned; ++i) rotate(row[i * GS * V * 4 + j], row[i * GS * V * 4 + j + half], cs[2 * j], cs[2 * j + 1]);
+    for (int j = gl; j < half && turned; j += GS)
+      for (int i = 0; i < n; ++i) rotate(row[i * GS * V * 4 + j], row[i * GS * V * 4 + j + half], cs[2 * j], cs[2 * j + 1]);
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < QK_HEADS; ++i)
@@ -556,48 +544,51 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rope_kernel(const KvVie
       for (int u = 0; u < V; ++u) e[i][u] = reinterpret_cast<float4*>(row + i * GS * V * 4)[gl + u * GS];
   }
 
-  // the same for where they go; pools are spaced by pages
-  uint16_t* q_to = a.q_out + static_cast<long long>(t) * a.n_heads * c.hd;
-  const long long slot = a.layer * c.layer_stride + page * c.page_stride + (p & ((1 << c.ps_shift) - 1)) * c.hd;
-  const int page_head = c.hd << c.ps_shift;
-  uint16_t* k_to = c.k + slot - static_cast<long long>(a.n_heads) * page_head;
-  uint16_t* v_to = c.v + slot - static_cast<long long>(n_qk) * page_head;
+  if (!is_q && !live) return;
+  // queries one head after the other, keys and values a page's head apart
+  const int step = (is_q ? c.hd : c.hd << c.ps_shift) / 4;
+  uint16_t* to = is_q ? a.q_out + (static_cast<long long>(t) * a.n_heads + h0) * c.hd
+                      : (is_k ? c.k : c.v) + a.layer * c.layer_stride + page * c.page_stride +
+                            ((static_cast<long long>(h0) << c.ps_shift) + (p & ((1 << c.ps_shift) - 1))) * c.hd;
+  uint2* to2 = reinterpret_cast<uint2*>(to) + gl;
 #pragma unroll
   for (int i = 0; i < QK_HEADS; ++i) {
-    const int h = h0 + i;
-    if (h >= per_token || (h >= a.n_heads && !live)) break;
-    uint2* to = reinterpret_cast<uint2*>(h < a.n_heads ? q_to + h * c.hd : (h < n_qk ? k_to : v_to) + static_cast<long long>(h) * page_head) + gl;
 #pragma unroll
     for (int u = 0; u < V; ++u)
-      if (gl + u * GS < nv)
-        to[u * GS] = live ? make_uint2(pack16<T>(e[i][u].x, e[i][u].y), pack16<T>(e[i][u].z, e[i][u].w)) : make_uint2(0u, 0u);
+      if (i < n && gl + u * GS < nv)
+        to2[u * GS] = live ? make_uint2(pack16<T>(e[i][u].x, e[i][u].y), pack16<T>(e[i][u].z, e[i][u].w)) : make_uint2(0u, 0u);
+    to2 += step;
   }
 }
 
-template <typename T, int GS, int V>
-cudaError_t launch_heads_as(const KvView& c, QkArgs a, cudaStream_t st) {
-  const int at_once = QK_HEADS * (32 / GS);
-  const int units = (a.n_heads + 2 * c.n_kv + at_once - 1) / at_once;
+template <typename T, int GS, int V, Turn TURN>
+cudaError_t launch_heads_as(const KvView& c, const QkArgs& a, cudaStream_t st) {
+  const int groups = (a.n_heads + QK_HEADS - 1) / QK_HEADS + 2 * ((c.n_kv + QK_HEADS - 1) / QK_HEADS);
+  const int units = (groups + 32 / GS - 1) / (32 / GS);  // warps a token
   const long long blocks = (static_cast<long long>(a.n_tokens) * units + QK_WARPS - 1) / QK_WARPS;
-  if (blocks > INT_MAX / QK_WARPS) return cudaErrorInvalidValue;  // units are counted in 32 bits
-  if (a.rope == nullptr)
-    a.form = QkArgs::NONE;
-  else if (!a.halves)
-    a.form = QkArgs::IN_LANE;
-  else
-    a.form = V == 1 && a.rot % 8 == 0 ? QkArgs::BETWEEN_LANES : QkArgs::IN_SHARED;
-  const size_t smem = a.form == QkArgs::IN_SHARED ? static_cast<size_t>(QK_WARPS) * 32 * V * QK_HEADS * 16 : 0;
-  if (smem > 48 * 1024) {
-    static const cudaError_t set =
-        cudaFuncSetAttribute(qk_norm_rope_kernel<T, GS, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, QK_WARPS * 32 * V * QK_HEADS * 16);
+  if (blocks > INT_MAX / QK_WARPS) return cudaErrorInvalidValue;  // warps are counted in 32 bits
+  constexpr size_t SMEM = TURN == Turn::InShared ? static_cast<size_t>(QK_WARPS) * 32 * V * QK_HEADS * 16 : 0;
+  if (SMEM > 48 * 1024) {
+    static const cudaError_t set = allow_smem(qk_norm_rope_kernel<T, GS, V, TURN>, SMEM);
     if (set != cudaSuccess) return set;
   }
-  return launch_dependent(qk_norm_rope_kernel<T, GS, V>, dim3(static_cast<unsigned>(blocks)), dim3(QK_WARPS * 32), smem, st, c, a, units);
+  return launch_dependent(qk_norm_rope_kernel<T, GS, V, TURN>, dim3(static_cast<unsigned>(blocks)), dim3(QK_WARPS * 32), SMEM, st, c, a, units);
+}
+
+template <typename T, int GS, int V>
+cudaError_t launch_heads_turned(const KvView& c, const QkArgs& a, cudaStream_t st) {
+  if (a.rope == nullptr) return launch_heads_as<T, GS, V, Turn::None>(c, a, st);
+  if (!a.halves) return launch_heads_as<T, GS, V, Turn::InLane>(c, a, st);
+  if constexpr (V == 1)
+    if (a.rot % 8 == 0) return launch_heads_as<T, GS, V, Turn::BetweenLanes>(c, a, st);
+  return launch_heads_as<T, GS, V, Turn::InShared>(c, a, st);
 }
 
 template <typename T>
 cudaError_t launch_heads(const KvView& c, const QkArgs& a, cudaStream_t st) {
-  return c.hd <= 64 ? launch_heads_as<T, 16, 1>(c, a, st) : c.hd <= 128 ? launch_heads_as<T, 32, 1>(c, a, st) : launch_heads_as<T, 32, 2>(c, a, st);
+  return c.hd <= 64    ? launch_heads_turned<T, 16, 1>(c, a, st)
+         : c.hd <= 128 ? launch_heads_turned<T, 32, 1>(c, a, st)
+                       : launch_heads_turned<T, 32, 2>(c, a, st);
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -737,7 +728,7 @@ int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   if (n_tokens == 0) return 1;
   const ex::QkArgs a{q, k, v, q_stride, k_stride, v_stride, n_tokens, n_heads, layer, q_weight, k_weight, eps, 1.0f / static_cast<float>(c.hd), rope,
                      rope_positions, rope_dims, rope_pairing == EDGEXPU_CUDA_ROPE_HALVES, seqs, pos,
-                     static_cast<uint16_t*>(q_out), ex::QkArgs::NONE};
+                     static_cast<uint16_t*>(q_out)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return ex::launched(cache->type == ex::TYPE_F16 ? ex::launch_heads<__half>(c, a, st) : ex::launch_heads<__nv_bfloat16>(c, a, st),
                       "qk_norm_rope");
