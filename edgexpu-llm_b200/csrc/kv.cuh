@@ -69,7 +69,7 @@ __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t v) {
 }
 
 template <typename T>
-__host__ __device__ constexpr uint32_t exponent16();  // the bits of the exponent
+__host__ __device__ constexpr uint32_t exponent16();  // the bits of the exponent, all ones in infinities and NaN
 template <>
 __host__ __device__ constexpr uint32_t exponent16<__half>() {
   return 0x7C00u;
@@ -77,17 +77,6 @@ __host__ __device__ constexpr uint32_t exponent16<__half>() {
 template <>
 __host__ __device__ constexpr uint32_t exponent16<__nv_bfloat16>() {
   return 0x7F80u;
-}
-
-// Whether eight values are all numbers: an exponent of all ones is an infinity or NaN.
-template <typename T>
-__device__ __forceinline__ bool finite16(const uint4& v) {
-  constexpr uint32_t e = exponent16<T>();
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  bool ok = true;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) ok = ok && (w[i] & e) != e && (w[i] & (e << 16)) != (e << 16);
-  return ok;
 }
 
 // Two weights >= 0 as a coarse number of the type each and the rest, both above 0 where the weight is (a

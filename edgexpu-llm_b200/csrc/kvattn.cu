@@ -40,6 +40,52 @@ struct RowsLayout {
   static_assert(JOIN_BYTES <= SLOTS * SLOT, "the join fits the ring");
 };
 
+// Row r of entry e (or of the batch, in the prefix) against tiles [t_begin, t_end), by one warp: a lane has
+// elements lane + 32 x, and a position it does not see is not read.
+template <typename T>
+__device__ __noinline__ void row_again(const AttnArgs& a, const Entry& e, int kvh, int r, int t_begin, int t_end, int pre, bool whole, int slot) {
+  const int lane = threadIdx.x & 31, hd = a.c.hd, tok = e.t0 + r / a.rep;
+  const long long row = static_cast<long long>(tok) * a.n_heads + kvh * a.rep + r % a.rep;
+  const int hi = pre ? e.len : e.len - e.nq + r / a.rep + 1;
+  const int32_t* table = a.c.table + static_cast<long long>(e.row) * a.c.max_pages;
+  auto value = [&](const uint16_t* base, int p, int d) {
+    const int page = min(max(table[p >> a.c.ps_shift], 0), a.c.n_pages - 1);
+    const uint16_t* at = base + a.layer_off + page * a.c.page_stride +
+                         ((static_cast<long long>(kvh) << a.c.ps_shift) + (p & ((1 << a.c.ps_shift) - 1))) * hd + d;
+    return unpack16<T>(*at).x;
+  };
+  float m = -INFINITY, l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p = max(e.start, t_begin * TILE); p < min(hi, t_end * TILE); ++p) {
+    float s = 0.0f;
+    for (int d = lane; d < hd; d += 32) s = fmaf(unpack16<T>(a.q[row * hd + d]).x, value(a.c.k, p, d), s);
+#pragma unroll
+    for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, y);
+    s *= a.scale;
+    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn, f = exp2f(m - base), w = exp2f(s - base + P_SHIFT);
+    m = mn;
+    l = l * f + w;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (lane + 32 * x < hd) o[x] = o[x] * f + w * value(a.c.v, p, lane + 32 * x);
+  }
+  const long long part = static_cast<long long>(slot) * a.n_tokens * a.n_heads + row;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const int d = lane + 32 * x;
+    if (d >= hd) continue;
+    if (!whole) {
+      a.part_o[part * hd + d] = o[x];
+    } else {
+      const float v = hi > 0 ? o[x] / l : 0.0f;
+      if (a.out_f32)
+        static_cast<float*>(a.out)[row * hd + d] = v;
+      else
+        static_cast<uint16_t*>(a.out)[row * hd + d] = round16<T>(v);
+    }
+  }
+  if (!whole && lane == 0) a.part_ml[part] = make_float2(m, l);
+}
+
 // One block: 16 * WM rows of one key/value head against one part of the prefix (PRE) or of an entry's
 // own positions.  Warp 4 brings K and V by TMA (128-byte swizzle; dims past head_dim read as 0).  Of the
 // other four, with WM = 4 each has 16 rows and all positions of a tile, with WM = 1 all have the same 16
@@ -47,12 +93,12 @@ struct RowsLayout {
 // product, as the tensor cores take it (with WM = 1, where bytes bound, in two numbers of the type); its
 // sum l is of the unrounded values.
 template <typename T, int DP, int WM>
-__global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
-    attn_rows_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const int pre) {
+__global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 3)
+    attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const int pre) {
   using L = RowsLayout<DP, WM>;
   constexpr int ROWS = L::ROWS, NT = WM == 1 ? 2 : 8, CH = DP / 8, ST = L::SLOTS;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ unsigned long long bad_keys;
+  __shared__ int any_odd;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t* empty = full + ST;
@@ -167,16 +213,24 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
     hi[h] = e.row < 0 ? 0 : pre ? shared : e.len - e.nq + r / rep + 1;
   }
   {
-    // a thread takes one chunk of eight elements of every (128 / CH)th row; rows past the end are the last
+    // a thread takes one chunk of eight elements of every (128 / CH)th row; rows past the end are 0
     constexpr int EACH = ROWS * CH / 128, STEP = ROWS / EACH;
     const int ch = threadIdx.x % CH;
     uint4 v[EACH];
+    const int dq = STEP / rep, dr = STEP - dq * rep;
+    int r = threadIdx.x / CH, tok_r = (r0 + r) / rep, g = r0 + r - tok_r * rep;
 #pragma unroll
     for (int x = 0; x < EACH; ++x) {
-      const int rr = r0 + min(static_cast<int>(threadIdx.x) / CH + x * STEP, n_rows - 1);
-      v[x] = ch * 8 < hd ? *reinterpret_cast<const uint4*>(
-                               a.q + (static_cast<long long>(e.t0 + rr / rep) * a.n_heads + kvh * rep + rr % rep) * hd + ch * 8)
-                         : make_uint4(0u, 0u, 0u, 0u);
+      v[x] = ch * 8 < hd && r < n_rows ? *reinterpret_cast<const uint4*>(
+                                             a.q + (static_cast<long long>(e.t0 + tok_r) * a.n_heads + kvh * rep + g) * hd + ch * 8)
+                                       : make_uint4(0u, 0u, 0u, 0u);
+      r += STEP;
+      tok_r += dq;
+      g += dr;
+      if (g >= rep) {
+        g -= rep;
+        ++tok_r;
+      }
     }
 #pragma unroll
     for (int x = 0; x < EACH; ++x) {
@@ -195,7 +249,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
 
   // A given-up wait does not leave the loop: its barriers are all four warps'.  What follows it is void,
   // and the status says so.
-  bool ok = true;
+  bool ok = true, odd = false;
   Ring<ST> ring;
   for (int t = t_begin; t < t_end; ++t) {
     ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
@@ -258,52 +312,20 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        s[i][x] = exp2f(s[i][x] - (base[x >> 1] - P_SHIFT));
+        s[i][x] = ex2(s[i][x] - (base[x >> 1] - P_SHIFT));
         l[x >> 1] += s[i][x];
       }
     ok = ok && __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag));
-    // A value that is no number, at a position that only some of the rows see: a product with a weight of
-    // 0 would spread it to the others, so it is added to the rows that see it and cleared for the product.
+    // values that are no numbers, at positions that only some of the rows see
     if (masked && block_lo_hi < block_hi) {
-      unsigned long long bad = 0;
       const int from = max(0, block_lo_hi - t * TILE), n = min(TILE, block_hi - t * TILE) - from;
+      uint32_t most = 0;  // the largest magnitudes, as 16-bit integers
       for (int x = threadIdx.x; x < n * CH; x += 128) {
         const int key = from + x / CH, ch = x % CH;
         const uint4 v = *reinterpret_cast<const uint4*>(vp + (ch >> 3) * L::HALF + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
-        if (!finite16<T>(v)) bad |= 1ull << key;
+        most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
       }
-      if (threadIdx.x == 0) bad_keys = 0;
-      named_bar_sync(1, 128);
-      if (bad != 0) atomicOr(&bad_keys, bad);
-      named_bar_sync(1, 128);
-      if (bad_keys != 0) {
-        bad = bad_keys;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-          for (int x = 0; x < 8; ++x) {
-            const int key = kw + i * 8 + x, p = t * TILE + key;
-            if (((bad >> key) & 1) == 0) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float pr = __shfl_sync(0xFFFFFFFFu, (x & 1) != 0 ? s[i][2 * h + 1] : s[i][2 * h], (lane & ~3) | (x >> 1));
-              if (p >= hi[h]) continue;
-#pragma unroll
-              for (int d = 0; d < DP / 8; ++d) {
-                const float2 v = unpack16<T>(*reinterpret_cast<const uint32_t*>(
-                    vp + (d >> 3) * L::HALF + key * 128 + (((d & 7) ^ (key & 7)) << 4) + (lane & 3) * 4));
-                o[d][2 * h] += pr * v.x;
-                o[d][2 * h + 1] += pr * v.y;
-              }
-            }
-          }
-        named_bar_sync(1, 128);
-        for (int x = threadIdx.x; x < n * CH; x += 128) {
-          const int key = from + x / CH, ch = x % CH;
-          if (((bad >> key) & 1) != 0) *reinterpret_cast<uint4*>(vp + (ch >> 3) * L::HALF + key * 128 + ((ch & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into it
-        named_bar_sync(1, 128);
-      }
+      if ((most & 0xFFFFu) >= exponent16<T>() || (most >> 16) >= exponent16<T>()) odd = true;
     }
     // positions that are not the block's hold anything: their values count as 0
     const bool edge = t * TILE < e.start || (t + 1) * TILE > block_hi;
@@ -350,7 +372,18 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
     *abort_flag = 1;
     atomicOr(a.c.status, ST_TIMEOUT_FULL);
   }
+  if (threadIdx.x == 0) any_odd = 0;
   named_bar_sync(1, 128);
+  if (odd) any_odd = 1;
+  named_bar_sync(1, 128);
+  if (any_odd != 0) {
+    // An infinity or NaN at a position that some rows do not see: its product with their weight of 0 has
+    // spread to them.  Rare, so these rows are simply computed again, one position after the other.
+    for (int r = w; r < n_rows; r += 4)
+      row_again<T>(a, e, kvh, r0 + r, t_begin, t_end, pre, whole, (pre ? 0 : a.n_pre) + split);
+    if (!pre) own_leave(a);
+    return;
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
@@ -421,8 +454,9 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : 3)
 }
 
 // Join the parts of each (token, head): a warp takes `heads` heads of a token, lane x elements 4 x ... and,
-// in wide heads, 4 x + 128 ...  The parts' weights come first, a lane a part, then their sums four at a time.
-template <typename T, bool WIDE>
+// in wide heads, 4 x + 128 ...  The parts' weights come first, a lane a part, then their sums AT_ONCE
+// at a time: eight where rows are few and latency counts, else four.
+template <typename T, bool WIDE, int AT_ONCE>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const int heads, const int per_token) {
   pdl_enter_grid();
   const int lane = threadIdx.x & 31, hd = a.c.hd;
@@ -500,10 +534,10 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
       // a part that saw nothing may not have written its sums
       uint32_t some = __ballot_sync(0xFFFFFFFFu, ml.x != -INFINITY || ml.y != 0.0f);
       while (some != 0) {
-        float4 v[4][WIDE ? 2 : 1];
-        float w[4];
+        float4 v[AT_ONCE][WIDE ? 2 : 1];
+        float w[AT_ONCE];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < AT_ONCE; ++x) {
           const int part = some != 0 ? __ffs(some) - 1 : -1;
           w[x] = __shfl_sync(0xFFFFFFFFu, f, max(part, 0));
           const float* src = a.part_o + row_of(b + max(part, 0)) * hd + lane * 4;
@@ -515,7 +549,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
           some &= some - 1;
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < AT_ONCE; ++x)
 #pragma unroll
           for (int k = 0; k < (WIDE ? 2 : 1); ++k) {
             o[k].x += w[x] * v[x][k].x;
@@ -641,7 +675,7 @@ cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, uint32_t t
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
   const int heads = rows <= 32LL * api_device_info().sm_count ? 1 : 4, per_token = (a.n_heads + heads - 1) / heads;
   const unsigned blocks = static_cast<unsigned>((static_cast<long long>(a.n_tokens) * per_token + 3) / 4);
-  return launch_dependent(a.c.hd > 128 ? attn_join_kernel<T, true> : attn_join_kernel<T, false>, dim3(blocks), dim3(128), 0, st, a,
+  return launch_dependent(a.c.hd > 128 ? attn_join_kernel<T, true, 4> : heads == 1 ? attn_join_kernel<T, false, 8> : attn_join_kernel<T, false, 4>, dim3(blocks), dim3(128), 0, st, a,
                           heads, per_token);
 }
 
