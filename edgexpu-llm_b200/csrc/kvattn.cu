@@ -589,14 +589,10 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
   const int own_tiles = (std::max(0, max_len - shared_len) + TILE - 1) / TILE + 1;
   p.one = !ragged && hd <= 128 && n_batch <= ONE_MAX_BATCH;
   p.n_own = 1;
-  if (p.one) {
-    // short runs and no prefix: a block each, which needs no join; a tile takes a block about 0.5 us, a join 3
-    const long long runs = static_cast<long long>(n_batch) * n_kv * ((rep + 15) / 16);
-    if ((shared_len > 0 || own_tiles > 8) && runs * own_tiles <= INT_MAX)
-      p.own_ctas = static_cast<int>(std::min(static_cast<long long>(attn_one_blocks(hd, rep, n_batch, runs * own_tiles)), runs * own_tiles));
-    else if (shared_len > 0)
-      p.one = false;
-  }
+  const long long runs = static_cast<long long>(n_batch) * n_kv * ((rep + 15) / 16);  // of single tokens
+  // short runs and no prefix: a block each, which needs no join; a tile takes a block about 0.5 us, a join 3
+  const bool cut = p.one && (shared_len > 0 || own_tiles > 8) && runs * own_tiles <= INT_MAX;
+  p.one = p.one && (cut || shared_len == 0);
   if (!p.one) {
     p.own_wm = rows <= 16LL * n_batch ? 1 : 4;
     const int own_rows = 16 * p.own_wm;
@@ -611,7 +607,17 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
     const int tiles = (shared_len + TC_TILE - 1) / TC_TILE;
     p.pre_rows = rows > 128 ? 256 : 128;
     const long long blocks = (rows + p.pre_rows - 1) / p.pre_rows * n_kv;
-    p.pre_ctas = static_cast<int>(std::min(static_cast<long long>(sms), blocks * tiles));
+    // Beside single tokens the shared pass takes its share of the SMs, by measured costs of SM time: 2.6 us a tile of 256
+    // rows, 1.6 of 128, 0.5 a tile of the own passes (taken half as long as they may be), and a tenth more, since the own
+    // pass goes on where the shared one has ended.  128 behind 32k: 184 -> 169 us, 32 behind 4k: 37 -> 32.  Several
+    // tokens' own passes want all SMs after it instead (shares of 0.6 and 0.85 of them: 192 -> 256, 198 us).
+    double share = 1.0;
+    if (p.one) {
+      const double pre = static_cast<double>(blocks) * tiles * (p.pre_rows == 256 ? 2.6 : 1.6);
+      const double own = 0.25 * runs * own_tiles;
+      share = std::min(1.0, std::max(0.35, 1.1 * pre / (pre + own)));
+    }
+    p.pre_ctas = static_cast<int>(std::min(static_cast<long long>(sms * share), blocks * tiles));
     p.n_pre = static_cast<int>(std::min(static_cast<long long>(tiles), p.pre_ctas / blocks + 2));
   } else if (shared_len > 0) {
     p.pre_wm = rows <= 16 ? 1 : 4;
@@ -619,6 +625,10 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
     const int tiles = (shared_len + TILE - 1) / TILE;
     const long long n = 2LL * sms / (static_cast<long long>(p.pre_blocks) * n_kv);
     p.n_pre = static_cast<int>(std::max(1LL, std::min({n, static_cast<long long>((tiles + 1) / 2), static_cast<long long>(MAX_SLOTS)})));
+  }
+  if (cut) {
+    const int free_sms = p.pre_ctas < sms ? sms - p.pre_ctas : sms;
+    p.own_ctas = static_cast<int>(std::min(static_cast<long long>(attn_one_blocks(hd, rep, n_batch, runs * own_tiles, free_sms)), runs * own_tiles));
   }
   return p;
 }

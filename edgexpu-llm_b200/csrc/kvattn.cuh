@@ -140,7 +140,7 @@ bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t 
 // Launch the single tokens' own pass (kvattn_one.cu), hd at most 128; its blocks where the line is cut.
 constexpr int ONE_MAX_BATCH = 2048;  // the runs' offsets are in shared memory
 cudaError_t launch_attn_one(const AttnArgs& a, uint32_t type, cudaStream_t st);
-int attn_one_blocks(int hd, int rep, int n_batch, long long tiles);
+int attn_one_blocks(int hd, int rep, int n_batch, long long tiles, int free_sms);
 
 // A place in a ring of slots, and the parity of its filling.
 template <int NS>

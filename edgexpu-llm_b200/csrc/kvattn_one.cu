@@ -355,13 +355,14 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
   own_leave(a);
 }
 
-// One round of blocks, or two where they get at least 16 tiles each: SMs do not get the same share of a busy
-// memory, and the second round evens that out (128 sequences of 33 to 2000 positions: 185 -> 182 us).
+// Two rounds of blocks: SMs do not get the same share of a busy memory, and the second round evens that out.
+// Of all SMs where each block gets 16 tiles and more (128 sequences of 33 to 2000 positions: one round 185
+// us, two 182), else of those that the shared pass leaves (32 behind 4k: one round 35.6 us, two 32.4).
 template <int DP>
-int blocks_of(int rep, int n_batch, long long tiles) {
+int blocks_of(int rep, int n_batch, long long tiles, int free_sms) {
   const size_t smem = one_smem<DP>(std::min(16, rep), n_batch, false);
-  const int round = std::max(1, std::min(static_cast<int>((228 * 1024) / (smem + 1024)), 2)) * api_device_info().sm_count;
-  return tiles >= 32LL * round ? 2 * round : round;
+  const int fit = std::max(1, std::min(static_cast<int>((228 * 1024) / (smem + 1024)), 2)), all = fit * api_device_info().sm_count;
+  return 2 * (tiles >= 32LL * all ? all : fit * free_sms);
 }
 
 template <typename T, int DP>
@@ -377,8 +378,8 @@ cudaError_t launch_one_as(const AttnArgs& a, uint32_t type, int blocks, cudaStre
 
 }  // namespace
 
-int attn_one_blocks(int hd, int rep, int n_batch, long long tiles) {
-  return hd <= 64 ? blocks_of<64>(rep, n_batch, tiles) : blocks_of<128>(rep, n_batch, tiles);
+int attn_one_blocks(int hd, int rep, int n_batch, long long tiles, int free_sms) {
+  return hd <= 64 ? blocks_of<64>(rep, n_batch, tiles, free_sms) : blocks_of<128>(rep, n_batch, tiles, free_sms);
 }
 
 cudaError_t launch_attn_one(const AttnArgs& a, uint32_t type, cudaStream_t st) {
