@@ -71,15 +71,14 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(const KvView c, const int3
   const int b = blockIdx.x, s = src[b], d = dst[b];
   if (d < 0) return;
   int bad = s < 0 || s >= c.n_seqs || d >= c.n_seqs;
+  const int held = bad ? 0 : c.lens[d], len = bad ? 0 : max(0, c.lens[s]);
   for (int j = threadIdx.x; j < n && !bad; j += blockDim.x) bad = (j < b && dst[j] == d) || dst[j] == s;
-  bad = __syncthreads_or(bad);
-  if (!bad) bad = c.lens[d] != 0;
+  bad = __syncthreads_or(bad || held != 0);
   if (bad) {
     if (threadIdx.x == 0) atomicOr(c.status, ST_BAD_CACHE);
     return;
   }
-  __syncthreads();  // every thread has read lens[d]
-  const int len = max(0, c.lens[s]), pages = min(kv_pages_of(c, len), c.max_pages);
+  const int pages = min(kv_pages_of(c, len), c.max_pages);
   const int32_t* from = c.table + static_cast<long long>(s) * c.max_pages;
   int32_t* to = c.table + static_cast<long long>(d) * c.max_pages;
   for (int i = threadIdx.x; i < pages; i += blockDim.x) {
@@ -122,9 +121,9 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   return r;
 }
 
-// The indices i in [from, to) with (refs[i] > 0) == live, ascending, into list[at ...) (list nullable);
-// stops once `most` are found.  Returns how many of them there are up to where it stopped.  All
-// threads of the block call it.
+// The first `most` indices i in [from, to) with (refs[i] > 0) == live, ascending, into list (nullable).
+// Returns how many there are up to where it stopped, which is after `most` of them.  All threads of the
+// block call it.
 __device__ int find_pages(const int32_t* refs, int from, int to, bool live, int most, int32_t* list, int* red) {
   constexpr int UN = 8;  // loads in flight a thread
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -147,7 +146,8 @@ __device__ int find_pages(const int32_t* refs, int from, int to, bool live, int 
     if (list != nullptr) {
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
-        if ((hit[u] >> lane) & 1u) list[off + __popc(hit[u] & ((1u << lane) - 1u))] = b + u * 32;
+        const int at = off + __popc(hit[u] & ((1u << lane) - 1u));
+        if (((hit[u] >> lane) & 1u) != 0 && at < most) list[at] = b + u * 32;
         off += __popc(hit[u]);
       }
     }
@@ -158,65 +158,103 @@ __device__ int find_pages(const int32_t* refs, int from, int to, bool live, int 
 
 // ---- taking -------------------------------------------------------------------------------------------
 
-// One block: what each entry needs, the lowest free pages for it, and the last pages to be copied.
-// With 64 sequences it is bound by latency (a chain of dependent loads and block barriers).
-__global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvView c, const int32_t* seqs,
-                                                                      const int32_t* n_new, int n, int32_t* pos,
-                                                                      int32_t* missing) {
-  pdl_enter_grid();
-  constexpr int PER = APPEND_MAX / PLAN_THREADS;
-  __shared__ int s_first[APPEND_MAX], s_off[APPEND_MAX + 1];  // an entry's first new column, its first place in the list
+// One block: what each entry needs, the lowest free pages for it, and the last pages to be copied.  Bound by
+// latency, a chain of dependent loads and block barriers.  FEW: at most 256 entries, one a thread; which
+// entry names a sequence first and which rows of the batch share a last page is then found by comparing
+// all pairs in shared memory, else by atomics in `work` (64 entries: 8 us there, 5 here).
+constexpr int APPEND_FEW = 256;
+constexpr int LIST_SHARED = 2048;  // pages found, in shared memory up to so many
+
+template <bool FEW>
+__global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvView c, const int32_t* seqs, const int32_t* n_new, int n,
+                                                                      int32_t* pos, int32_t* missing) {
+  constexpr int PER = FEW ? 1 : APPEND_MAX / PLAN_THREADS, MOST = FEW ? APPEND_FEW : APPEND_MAX;
+  __shared__ int s_first[MOST], s_off[MOST + 1];  // an entry's first new column, its first place in the list
+  __shared__ int s_seq[FEW ? MOST : 1], s_tail[FEW ? MOST : 1];
+  __shared__ int s_list[FEW ? LIST_SHARED : 1];
   __shared__ int red[33];
   __shared__ int n_jobs;
   const Work w = work_of(c);
+  const int in_page = (1 << c.ps_shift) - 1;
   if (threadIdx.x == 0) n_jobs = 0;
-  // a sequence belongs to the first entry that names it
-  for (int b = threadIdx.x; b < n; b += blockDim.x)
-    if (seqs[b] >= 0 && seqs[b] < c.n_seqs) w.owner[seqs[b]] = INT_MAX;
-  __syncthreads();
-  for (int b = threadIdx.x; b < n; b += blockDim.x)
-    if (seqs[b] >= 0 && seqs[b] < c.n_seqs) atomicMin(&w.owner[seqs[b]], b);
-  __syncthreads();
-  // entries 4 * thread ..., so that a scan over threads is a scan over the batch
-  int len[PER], add[PER], tail[PER];  // tail: the page that holds the last tokens, when it has room; else -1
+  pdl_enter_grid();
+  int seq[PER], len[PER], add[PER], tail[PER];  // tail: the page that holds the last tokens, when it has room; else -1
+  bool ok[PER];
+  // entries PER * thread ..., so that a scan over threads is a scan over the batch
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int b = threadIdx.x * PER + e;
-    len[e] = add[e] = tail[e] = -1;
-    if (b >= n || seqs[b] < 0) continue;
-    const int s = seqs[b];
-    bool ok = s < c.n_seqs && w.owner[s] == b;
-    if (ok) {
-      const int held = c.lens[s], more = n_new[b];
-      ok = held >= 0 && more >= 0 && static_cast<long long>(held) + more <= (static_cast<long long>(c.max_pages) << c.ps_shift);
-      if (ok) {
-        len[e] = held;
-        add[e] = more;
-        if ((held & ((1 << c.ps_shift) - 1)) != 0 && more > 0) {
-          tail[e] = c.table[static_cast<long long>(s) * c.max_pages + (held >> c.ps_shift)];
-          if (tail[e] < 0 || tail[e] >= c.n_pages) {
-            ok = false;
-            len[e] = add[e] = tail[e] = -1;
-          }
+    seq[e] = b < n ? seqs[b] : -1;
+    add[e] = b < n ? n_new[b] : 0;
+    ok[e] = seq[e] >= 0 && seq[e] < c.n_seqs;
+    if (seq[e] >= c.n_seqs) atomicOr(c.status, ST_BAD_CACHE);
+    len[e] = ok[e] ? c.lens[seq[e]] : 0;
+    // a sequence belongs to the first entry that names it
+    if constexpr (FEW) {
+      if (b < n) s_seq[b] = seq[e];
+    } else if (ok[e]) {
+      w.owner[seq[e]] = INT_MAX;
+    }
+  }
+  __syncthreads();
+  if constexpr (FEW) {
+    const int b = threadIdx.x;
+    bool first = true;
+    if (ok[0])
+#pragma unroll 8
+      for (int j = 0; j < b; ++j) first &= s_seq[j] != seq[0];
+    if (ok[0] && !first) {
+      ok[0] = false;
+      atomicOr(c.status, ST_BAD_CACHE);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (ok[e]) atomicMin(&w.owner[seq[e]], static_cast<int>(threadIdx.x) * PER + e);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (ok[e] && w.owner[seq[e]] != static_cast<int>(threadIdx.x) * PER + e) {
+        ok[e] = false;
+        atomicOr(c.status, ST_BAD_CACHE);
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int b = threadIdx.x * PER + e;
+    tail[e] = -1;
+    if (ok[e]) {
+      bool fits = len[e] >= 0 && add[e] >= 0 && static_cast<long long>(len[e]) + add[e] <= (static_cast<long long>(c.max_pages) << c.ps_shift);
+      if (fits && (len[e] & in_page) != 0 && add[e] > 0) {
+        tail[e] = c.table[static_cast<long long>(seq[e]) * c.max_pages + (len[e] >> c.ps_shift)];
+        if (tail[e] < 0 || tail[e] >= c.n_pages) {
+          fits = false;
+          tail[e] = -1;
         }
       }
+      ok[e] = fits;
+      if (!fits) atomicOr(c.status, ST_BAD_CACHE);
     }
-    if (!ok) atomicOr(c.status, ST_BAD_CACHE);
-    if (tail[e] >= 0) {
+    if constexpr (FEW) {
+      if (b < n) s_tail[b] = tail[e];
+    } else if (tail[e] >= 0) {
       w.count[tail[e]] = 0;
       w.last[tail[e]] = -1;
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < PER; ++e)
-    if (tail[e] >= 0) {
-      atomicAdd(&w.count[tail[e]], 1);
-      atomicMax(&w.last[tail[e]], static_cast<int>(threadIdx.x) * PER + e);
-    }
-  __syncthreads();
+  // a shared last page is copied, but for the last of the rows of the batch that share it when they are all its holders
   int need = 0, want[PER];
   bool split[PER];
+  if constexpr (!FEW) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (tail[e] >= 0) {
+        atomicAdd(&w.count[tail[e]], 1);
+        atomicMax(&w.last[tail[e]], static_cast<int>(threadIdx.x) * PER + e);
+      }
+    __syncthreads();
+  }
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int b = threadIdx.x * PER + e;
@@ -224,9 +262,23 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
     want[e] = 0;
     if (tail[e] >= 0) {
       const int r = c.refs[tail[e]];
-      split[e] = r > 1 && !(w.count[tail[e]] >= r && w.last[tail[e]] == b);
+      if (r > 1) {
+        int sharers = 0, last = -1;
+        if constexpr (FEW) {
+#pragma unroll 8
+          for (int j = 0; j < n; ++j) {
+            const bool alike = s_tail[j] == tail[e];
+            sharers += alike ? 1 : 0;
+            last = alike ? j : last;
+          }
+        } else {
+          sharers = w.count[tail[e]];
+          last = w.last[tail[e]];
+        }
+        split[e] = !(sharers >= r && last == b);
+      }
     }
-    if (add[e] >= 0) {
+    if (ok[e]) {
       s_first[b] = kv_pages_of(c, len[e]) - (split[e] ? 1 : 0);
       want[e] = kv_pages_of(c, len[e] + add[e]) - s_first[b];
       need += want[e];
@@ -241,17 +293,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
     off += want[e];
   }
   if (threadIdx.x == 0) s_off[n] = total;
-  const int found = total > 0 ? find_pages(c.refs, 0, c.n_pages, false, total, w.list, red) : 0;
+  int32_t* list = FEW && total <= LIST_SHARED ? s_list : w.list;
+  const int found = total > 0 ? find_pages(c.refs, 0, c.n_pages, false, total, list, red) : 0;
   const bool fits = found >= total;
   __syncthreads();
-  if (fits) {  // a warp an entry: its pages into its row
+  if (fits && total > 0) {  // a warp an entry: its pages into its row
     const int lane = threadIdx.x & 31;
     for (int b = threadIdx.x >> 5; b < n; b += blockDim.x >> 5) {
       const int at = s_off[b], take = s_off[b + 1] - at;
       if (take == 0) continue;
       int32_t* row = c.table + static_cast<long long>(seqs[b]) * c.max_pages + s_first[b];
       for (int i = lane; i < take; i += 32) {
-        const int p = w.list[at + i];
+        const int p = list[at + i];
         row[i] = p;
         c.refs[p] = 1;
       }
@@ -261,16 +314,16 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
   for (int e = 0; e < PER; ++e) {
     const int b = threadIdx.x * PER + e;
     if (b >= n) continue;
-    const bool done = fits && add[e] >= 0;
+    const bool done = fits && ok[e];
     if (pos != nullptr) pos[b] = done ? len[e] : -1;
     if (!done) continue;
-    c.lens[seqs[b]] = len[e] + add[e];
+    c.lens[seq[e]] = len[e] + add[e];
     if (split[e]) {
       atomicSub(&c.refs[tail[e]], 1);
       const int j = atomicAdd(&n_jobs, 1);
       w.jobs[3 * j] = tail[e];
-      w.jobs[3 * j + 1] = w.list[s_off[b]];
-      w.jobs[3 * j + 2] = len[e] & ((1 << c.ps_shift) - 1);
+      w.jobs[3 * j + 1] = list[s_off[b]];
+      w.jobs[3 * j + 2] = len[e] & in_page;
     }
   }
   __syncthreads();
@@ -652,7 +705,7 @@ int edgexpu_cuda_kv_append_dev(const edgexpu_cuda_kv_cache* cache, const int32_t
   if (!ex::page_call(cache, "kv_append", true, n, n == 0 || (seqs != nullptr && n_new != nullptr), &c)) return 0;
   if (n > ex::APPEND_MAX) return ex::api_fail(nullptr, 0, "kv_append: %d entries (at most %d)", n, ex::APPEND_MAX);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = ex::launch_dependent(ex::kv_append_plan_kernel, dim3(1), dim3(ex::PLAN_THREADS), 0, st, c, seqs, n_new, n, pos, missing);
+  cudaError_t e = ex::launch_dependent(n <= ex::APPEND_FEW ? ex::kv_append_plan_kernel<true> : ex::kv_append_plan_kernel<false>, dim3(1), dim3(ex::PLAN_THREADS), 0, st, c, seqs, n_new, n, pos, missing);
   if (e == cudaSuccess && n > 0) {
     const ex::Work w = ex::work_of(c);
     const ex::MoveArgs a{w.jobs, w.jobs + 1, 3, 0, w.head, nullptr, nullptr};
