@@ -138,7 +138,7 @@ __device__ __forceinline__ float ex2(float x) {
 bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type);
 
 // Launch the single tokens' own pass (kvattn_one.cu), hd at most 128; its blocks where the line is cut.
-constexpr int ONE_MAX_BATCH = 2048;  // the runs' offsets are in shared memory
+constexpr int ONE_MAX_BATCH = 1024;  // what the runs need is in shared memory
 cudaError_t launch_attn_one(const AttnArgs& a, uint32_t type, cudaStream_t st);
 int attn_one_blocks(int hd, int rep, int n_batch, long long tiles, int free_sms);
 

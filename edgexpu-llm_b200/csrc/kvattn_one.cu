@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "capi_internal.h"
 #include "kvattn.cuh"
@@ -36,7 +37,7 @@ struct OneLayout {
 // Dynamic shared memory: ring, barriers, the four warps' sums for a run's join, the runs' offsets.
 template <int DP>
 size_t one_smem(int rows, int n_batch, bool whole) {
-  return OneLayout<DP>::FIXED + static_cast<size_t>(4) * rows * (DP + 2) * 4 + (whole ? 0 : (n_batch + 1) * 4) + 1024;
+  return OneLayout<DP>::FIXED + static_cast<size_t>(4) * rows * (DP + 2) * 4 + (whole ? 0 : (3 * n_batch + 1) * 4) + 1024;
 }
 
 struct Run {
@@ -61,6 +62,8 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
   float* join_o = reinterpret_cast<float*>(smem + L::FIXED);             // [warp][rows16][DP]
   float* join_ml = join_o + 4 * rows16 * DP;                             // [warp][rows16][m, l]
   int* off = reinterpret_cast<int*>(join_ml + 4 * rows16 * 2);           // [n_batch + 1]: tiles before an entry's run
+  int* lens = off + a.n_batch + 1;                                       // [n_batch]: its length, ~length where it shares the prefix
+  int* table_row = lens + a.n_batch;                                     // [n_batch]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -87,6 +90,8 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
     for (int i = from; i < to; ++i) {
       const Entry e = entry_of(a, i, shared);
       off[i] = mine;
+      lens[i] = e.shares ? ~e.len : e.len;
+      table_row[i] = e.row;
       mine += cut_of(e.start, e.len, 1).tiles;
     }
     int inc = mine;
@@ -111,7 +116,8 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
       off[a.n_batch] = all;
       if (blockIdx.x == 0) a.own_off[a.n_batch] = all;
     }
-    const long long total = static_cast<long long>(all) * per_entry, per = (total + a.own_ctas - 1) / a.own_ctas;
+    const long long total = static_cast<long long>(all) * per_entry;
+    const long long per = total <= INT_MAX / 2 ? (static_cast<int>(total) + a.own_ctas - 1) / a.own_ctas : (total + a.own_ctas - 1) / a.own_ctas;
     begin = blockIdx.x * per;
     end = min(total, begin + per);
   }
@@ -129,23 +135,26 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
   auto run_at = [&](long long at, int& i) {
     Run r;
     if (whole) {
+      const Entry e = entry_of(a, first_entry, shared);
       r.entry = first_entry;
+      r.row = e.row;
+      r.len = e.len;
+      r.start = e.start;
     } else {
       while (static_cast<long long>(off[i + 1]) * per_entry <= at) ++i;
       r.entry = i;
+      r.row = table_row[i];
+      r.len = lens[i] < 0 ? ~lens[i] : lens[i];
+      r.start = lens[i] < 0 ? shared : 0;
     }
-    const Entry e = entry_of(a, r.entry, shared);
-    r.row = e.row;
-    r.len = e.len;
-    r.start = e.start;
-    const Cut cut = cut_of(e.start, e.len, 1);
+    const Cut cut = cut_of(r.start, r.len, 1);
     int which, t = 0;
     r.n = cut.tiles;
     if (whole) {
       which = blockIdx.x % per_entry;
     } else {
-      const long long in = at - static_cast<long long>(off[r.entry]) * per_entry;
-      which = static_cast<int>(in / cut.tiles);
+      const long long in = at - static_cast<long long>(off[i]) * per_entry;
+      which = in <= INT_MAX ? static_cast<int>(in) / cut.tiles : static_cast<int>(in / cut.tiles);
       t = static_cast<int>(in - static_cast<long long>(which) * cut.tiles);
       r.n = static_cast<int>(min(static_cast<long long>(cut.tiles - t), end - at));
     }

@@ -247,14 +247,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       drain<NS>(ring, issued, full, a.c.status);
     }
   } else if (warp == 1) {
-    // The warp runs the loop together and one thread issues: descriptors are then uniform where they are made.
+    // One elected thread: each wait and each turn of a whole warp costs it about 100 ns between products.
     const uint32_t q_s = smem_u32(smem), ring_s = smem_u32(smem + L::RING);
-    const bool lead = elect_one();
+    if (elect_one()) {
     Ring<NS> v;  // V of the tile in use; K of the next one is the place after it
     v.next();
     uint32_t segs = 0, par[2] = {0, 0};  // parity of either buffer's next P; constant indices only
     bool ok = true;
-    auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, spin(bar, parity, abort_flag)) != 0; };
+    auto there = [&](uint64_t* bar, uint32_t parity) { return spin(bar, parity, abort_flag); };
     // S of 64 positions, the first or last of a tile, into the buffer of that parity
     auto product_s = [&](int half, uint32_t kd, int b) {
       const uint32_t qd = sw128_desc(q_s + half * L::SLOT, 16);
@@ -275,16 +275,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int h = 0; h < MT; ++h) ok = ok && there(&q_full[h], segs & 1u);
       if (!ok) break;
       tc_after();
-      if (lead) {
-        const uint32_t kd = sw128_desc(ring_s + k.slot * L::SLOT, 16);
+      const uint32_t kd0 = sw128_desc(ring_s + k.slot * L::SLOT, 16);
 #pragma unroll
-        for (int h = 0; h < MT; ++h) product_s(h, kd, 0);
-        if (g.steps > 1)
+      for (int h = 0; h < MT; ++h) product_s(h, kd0, 0);
+      if (g.steps > 1)
 #pragma unroll
-          for (int h = 0; h < MT; ++h) product_s(h, kd, 1);
-        tc_commit(&empty[k.slot]);
-      }
-      __syncwarp();
+        for (int h = 0; h < MT; ++h) product_s(h, kd0, 1);
+      tc_commit(&empty[k.slot]);
       for (int j = 0; ok && j < g.steps; j += 2) {
         k.next();
         k.next();
@@ -299,40 +296,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             ok = ok && there(&p_full[2 * h + b], par[b]);
             if (!ok) break;
             tc_after();
-            if (lead) {
-              const uint32_t p_at = tmem + 128 * h + STEP * b;
+            const uint32_t p_at = tmem + 128 * h + STEP * b;
 #pragma unroll
-              for (int s = 0; s < STEP / 16; ++s) {
-                const uint32_t vs = vd0 + ((b * STEP * 128 + s * 2048) >> 4);
-                mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, b > 0 || s > 0 || j > 0);
-                if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
-              }
-              tc_commit(&o_done[2 * h + b]);
+            for (int s = 0; s < STEP / 16; ++s) {
+              const uint32_t vs = vd0 + ((b * STEP * 128 + s * 2048) >> 4);
+              mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, b > 0 || s > 0 || j > 0);
+              if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
             }
-            __syncwarp();
+            tc_commit(&o_done[2 * h + b]);
             if (more && b == 0 && h == 0) ok = there(&full[k.slot], k.phase);
             if (!ok) break;
-            if (more && lead) product_s(h, kd, b);
-            __syncwarp();
+            if (more) product_s(h, kd, b);
           }
           par[b] ^= 1u;
         }
-        if (lead) {  // both tiles' places are free once these products are done
-          tc_commit(&empty[v.slot]);
-          if (j + 2 < g.steps) tc_commit(&empty[k.slot]);
-        }
-        __syncwarp();
+        tc_commit(&empty[v.slot]);  // both tiles' places are free once these products are done
+        if (j + 2 < g.steps) tc_commit(&empty[k.slot]);
         v.next();
         v.next();
       }
     }
-    if (lead) {
-      if (!ok) {
-        *abort_flag = 1;
-        atomicOr(a.c.status, ST_TIMEOUT_FULL);
-      }
-      tc_commit(fin);  // all products are done before tensor memory is given back
-      if (!mbar_wait(fin, 0)) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
+    if (!ok) {
+      *abort_flag = 1;
+      atomicOr(a.c.status, ST_TIMEOUT_FULL);
+    }
+    tc_commit(fin);  // all products are done before tensor memory is given back
+    if (!mbar_wait(fin, 0)) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
     }
     __syncwarp();
   } else if (warp >= 4 && warp < 4 + 4 * MT) {
