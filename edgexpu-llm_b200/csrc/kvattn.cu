@@ -11,6 +11,13 @@
 // zeros, so memory past a sequence's end may hold anything.  A sequence one of whose tokens sees less
 // than the whole prefix takes no part in the shared pass: its own pass starts at position 0, which
 // keeps the shared pass free of masks by row.
+//
+// Launches: the shared pass (kvattn_tc.cu; the rows kernel here for heads above 128 elements or at most
+// 16 rows), beside it the own pass (kvattn_one.cu for single tokens, else the rows kernel here), then the
+// join.  Floor: K and V of the prefix and of each sequence once, or 4 operations an element of K for each
+// row.  Measured, 32 query heads on 8 of 128 elements in bf16: 128 single tokens behind a prefix of 32k
+// with 33 to 2000 own positions 160 us (floor 101, bytes), 32 behind 4k with up to 511 32 us (8, bytes;
+// three kernels' latencies), 32 questions of 1 to 64 tokens behind 8k 187 us (84, operations).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -91,7 +98,9 @@ __device__ __noinline__ void row_again(const AttnArgs& a, const Entry& e, int kv
 // other four, with WM = 4 each has 16 rows and all positions of a tile, with WM = 1 all have the same 16
 // rows and 16 positions of each tile, and join at the end.  P is rounded to the cache's type for its
 // product, as the tensor cores take it (with WM = 1, where bytes bound, in two numbers of the type); its
-// sum l is of the unrounded values.
+// sum l is of the unrounded values.  Fragments of warp products, since an own pass has few rows on few
+// positions.  The own passes of 32 questions of 1 to 64 tokens on 64 to 200 positions: 41 us, bound by
+// latency, a tile's two products and its softmax in turn in each warp.
 template <typename T, int DP, int WM>
 __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 3)
     attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const int pre) {
@@ -455,7 +464,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 
 
 // Join the parts of each (token, head): a warp takes `heads` heads of a token, lane x elements 4 x ... and,
 // in wide heads, 4 x + 128 ...  The parts' weights come first, a lane a part, then their sums AT_ONCE
-// at a time: eight where rows are few and latency counts, else four.
+// at a time: eight where rows are few and latency counts, else four.  Bound by latency (4096 rows of four
+// parts: 10 to 15 us), with many rows by its instructions (32k rows: 27 us; issue slots 62 % in use).
 template <typename T, bool WIDE, int AT_ONCE>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const int heads, const int per_token) {
   pdl_enter_grid();
@@ -494,7 +504,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
     long long cont = 0;  // single tokens: the row of the second own part
     if (sees && e.shares) {
       if (a.pre_rows > 0) {
-        const int first = (kvh * pre.row_blocks + (t * a.rep + r) / a.pre_rows) * pre.tiles;
+        const int first = (kvh * pre.lines + (t * a.rep + r) / a.pre_rows / a.pre_width) * pre.tiles;
         n_pre = (first + pre.tiles - 1) / pre.per - first / pre.per + 1;
       } else {
         n_pre = cut_of(0, shared, a.n_pre).used;
@@ -575,7 +585,7 @@ struct AttnPlan {
   int pre_wm, own_wm;
   int pre_blocks, own_blocks;
   int n_pre, n_own;
-  int pre_rows, pre_ctas;
+  int pre_rows, pre_ctas, pre_width;
   bool one;      // single tokens: kvattn_one.cu
   int own_ctas;
 };
@@ -617,8 +627,15 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
       const double own = 0.25 * runs * own_tiles;
       share = std::min(1.0, std::max(0.35, 1.1 * pre / (pre + own)));
     }
-    p.pre_ctas = static_cast<int>(std::min(static_cast<long long>(sms * share), blocks * tiles));
-    p.n_pre = static_cast<int>(std::min(static_cast<long long>(tiles), p.pre_ctas / blocks + 2));
+    // The blocks of rows of a head go side by side along one piece where at least two pieces fit: with pieces of their
+    // own, the two of 128 behind 32k read 254 MB from HBM of a prefix of 134.  165 -> 161 us there, 189 -> 187 with sixteen.
+    const int limit = std::max(1, static_cast<int>(sms * share));
+    const long long row_blocks = blocks / n_kv;
+    p.pre_width = row_blocks <= limit / 2 ? static_cast<int>(row_blocks) : 1;
+    const long long lines = blocks / p.pre_width;
+    const int pieces = static_cast<int>(std::min(static_cast<long long>(limit / p.pre_width), lines * tiles));
+    p.pre_ctas = pieces * p.pre_width;
+    p.n_pre = static_cast<int>(std::min(static_cast<long long>(tiles), pieces / lines + 2));
   } else if (shared_len > 0) {
     p.pre_wm = rows <= 16 ? 1 : 4;
     p.pre_blocks = static_cast<int>((rows + 16 * p.pre_wm - 1) / (16 * p.pre_wm));
@@ -748,6 +765,7 @@ int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache* cache, int layer,
   a.n_own = p.n_own;
   a.pre_rows = p.pre_rows;
   a.pre_ctas = p.pre_ctas;
+  a.pre_width = p.pre_width;
   a.own_ctas = p.own_ctas;
   const size_t parts = static_cast<size_t>(ex::part_rows(p, n_tokens, n_heads));
   uint8_t* at = static_cast<uint8_t*>(work);

@@ -27,6 +27,7 @@ struct AttnArgs {
   int n_pre, n_own;  // parts of the shared prefix, and of a sequence's own positions
   int pre_rows;      // rows a block of the tensor-memory kernel's shared pass; 0: the rows kernel makes it
   int pre_ctas;      // its blocks
+  int pre_width;     // blocks that share a piece of its line
   int own_ctas;      // blocks of the single-token kernel, whose line of work is cut into equal pieces; 0: a run each
   int* own_off;      // [n_batch + 1]: tiles of the line before each entry's run (by the kernel, for the join)
   long long cont_row0;  // row of part_o, part_ml where the blocks' 16 continuing rows begin
@@ -103,19 +104,22 @@ __device__ __forceinline__ Cut cut_of(int start, int end, int n) {
   return c;
 }
 
-// The shared pass of the tensor-memory kernel.  Its blocks of rows (kv head outside, rows inside) times
-// the prefix's tiles are one line of work, cut into pre_ctas equal pieces; a block of rows is then
-// divided over the pieces that touch it, and piece c's part of it is slot c - (the first such piece).
+// The shared pass of the tensor-memory kernel.  (kv head, block of rows, tile of the prefix) is a line of
+// work cut into equal pieces.  Where a few blocks of rows make up a head, pre_width blocks of the grid, one
+// for each, take the same piece of the line (kv head, tile), so that what one of them brings from HBM the
+// others find in L2; else pre_width is 1 and the blocks of rows are in the line.  A block of rows is divided
+// over the pieces that touch it, and piece c's part of it is slot c - (the first such piece).
 constexpr int TC_TILE = 128;  // positions
 struct TcCut {
-  int tiles, row_blocks, total, per;
+  int tiles, lines, total, per;  // lines: blocks of rows of a head that are in the line
 };
 __device__ __forceinline__ TcCut tc_cut(const AttnArgs& a, int shared) {
   TcCut c;
   c.tiles = (shared + TC_TILE - 1) / TC_TILE;
-  c.row_blocks = (a.n_tokens * a.rep + a.pre_rows - 1) / a.pre_rows;
-  c.total = c.row_blocks * a.c.n_kv * c.tiles;
-  c.per = (c.total + a.pre_ctas - 1) / a.pre_ctas;
+  c.lines = (a.n_tokens * a.rep + a.pre_rows - 1) / a.pre_rows / a.pre_width;
+  c.total = c.lines * a.c.n_kv * c.tiles;
+  const int pieces = a.pre_ctas / a.pre_width;
+  c.per = (c.total + pieces - 1) / pieces;
   return c;
 }
 

@@ -9,8 +9,11 @@
 //
 // Warp 4 brings K and V by TMA (128-byte swizzle; dims past head_dim read as 0) through a ring that runs
 // on from one run to the next; warps 0..3 take 16 positions of each tile each, with Q and O in
-// registers, and meet only at a run's end.  Bound by HBM: K and V are read once, at 4 (heads of the
-// group) operations a byte.
+// registers, and meet only at a run's end.  P goes to its product in two numbers of the cache's type.
+//
+// Bound by HBM: K and V are read once, at (heads of the group) operations a byte.  128 sequences of 33 to
+// 2000 own positions, 8 heads of 128 elements: 543 MB in 104 us on all SMs, 5.2 TB/s; 32 sequences of 1
+// to 511: 45 MB in 21 us, where a block's first loads and its warps' join are a third.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -2,19 +2,26 @@
 // the queries of all sequences, stacked, against the prefix that they share.
 //
 // One block takes up to MT x 128 rows (tokens x heads of a key/value head's group) along its piece of
-// the prefix, 128 positions at a time.  Per tile and 128 rows: S = Q K^T into 128 columns of tensor
+// the prefix, in steps of 64 positions.  Per step and 128 rows: S = Q K^T into 64 columns of tensor
 // memory, one thread a row takes the row's maximum, exponentials and sum, writes P in the cache's type
-// over S, and O += P V accumulates in tensor memory with P as the tensor-memory operand.  With MT = 2
-// the products of one half of the rows run while the other half is in its softmax, and both read the
-// same tiles of K and V.  A row's reference maximum moves only when the maximum has grown by more than
-// GROW (in log2 units); then O and the sum are rescaled, which after the first tiles is rare.
+// over S, and O += P V accumulates in tensor memory with P as the tensor-memory operand.  Two buffers of
+// S a half of the rows, and two halves with MT = 2: products of one run while another is in its softmax,
+// and both halves read the same tiles of K and V.  A row's reference maximum moves only when the maximum
+// has grown by more than GROW (in log2 units); then O and the sum are rescaled, which after the first
+// tiles is rare.  P is rounded to the cache's type for its product (with MT = 1, where bytes bound, in
+// two numbers of the type); its sum l, S and O are fp32.
 //
 // Warps: 0 brings K and V by TMA (a box a page and 64 elements; 128-byte swizzle) through a ring of
-// slots, 1 issues the products, 4..7 and 8..11 are the rows.  S, P: columns 128 x; O: columns
-// 256 + 128 x of half x.  Tensor memory holds the whole accumulation, so shared memory is Q and the ring.
+// slots of 128 positions, one thread of 1 issues the products, 4..7 and 8..11 are the rows.  S, P:
+// columns 128 x + 64 b of half x and buffer b; O: columns 256 + 128 x.  Tensor memory holds the whole
+// accumulation, so shared memory is Q and the ring.
 //
-// Bound: per tile and 128 rows the two products take 2 x 512 cycles of the tensor pipe (head_dim 128)
-// and the exponentials 1024 of the special-function units, beside 64 KB of K and V from L2 or HBM.
+// Bound: 256 rows of head_dim 128 in 16 bits against 128 positions are 2 x 4 x 128 x 128 x 128 operations:
+// 1.5 us of an SM at the rate of a large library product.  Measured: about 2.4 us, the chain from the
+// softmax's P through the issuing thread to the next S; the tensor pipe is busy 49 % of the time for 4085
+// rows of each of 8 heads on 8k positions (152 us), 57 % for 512 rows of each on 32k (112 us on 90 SMs).  Measured and not taken: steps of 128 (one buffer: 147 -> 160 us), a ring of 64 positions
+// (twice the waits and commits: 140 -> 175), the halves' waits joined (175), exponentials by polynomial
+// on 1/8 to 1/2 of the columns (+1 to +4 %).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -152,14 +159,15 @@ struct Segment {
   int kvh, row0, tile0, n, slot;
   int steps;  // the prefix's last half tile may be empty
 };
-__device__ __forceinline__ Segment segment_at(const TcCut& c, int at, int end, int pre_rows, int shared) {
+__device__ __forceinline__ Segment segment_at(const TcCut& c, int at, int end, const AttnArgs& a, int shared) {
   Segment s;
   const int block = at / c.tiles;
   s.tile0 = at - block * c.tiles;
   s.n = min(c.tiles - s.tile0, end - at);
-  s.kvh = block / c.row_blocks;
-  s.row0 = (block - s.kvh * c.row_blocks) * pre_rows;
-  s.slot = static_cast<int>(blockIdx.x) - block * c.tiles / c.per;
+  s.kvh = block / c.lines;
+  const int piece = blockIdx.x / a.pre_width, in_piece = blockIdx.x - piece * a.pre_width;
+  s.row0 = ((block - s.kvh * c.lines) * a.pre_width + in_piece) * a.pre_rows;
+  s.slot = piece - block * c.tiles / c.per;
   s.steps = min(2 * s.n, (shared - s.tile0 * TC_TILE + STEP - 1) / STEP);
   return s;
 }
@@ -219,7 +227,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   const int shared = __shfl_sync(0xFFFFFFFFu, shared_of(a), 0);
   const TcCut cut = tc_cut(a, shared);
-  const int begin = min(cut.total, static_cast<int>(blockIdx.x) * cut.per), end = min(cut.total, begin + cut.per);
+  const int begin = min(cut.total, static_cast<int>(blockIdx.x) / a.pre_width * cut.per), end = min(cut.total, begin + cut.per);
 
   if (warp == 0) {
     // K of tile 0, V of tile 0, K of tile 1, ...: the order in which the products need them
@@ -228,7 +236,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     int issued = 0;
     bool ok = true;
     for (int at = begin; ok && at < end;) {
-      const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
+      const Segment g = segment_at(cut, at, end, a, shared);
       at += g.n;
       for (int i = 0; ok && i < 2 * g.n; ++i) {
         ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
@@ -250,78 +258,78 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     // One elected thread: each wait and each turn of a whole warp costs it about 100 ns between products.
     const uint32_t q_s = smem_u32(smem), ring_s = smem_u32(smem + L::RING);
     if (elect_one()) {
-    Ring<NS> v;  // V of the tile in use; K of the next one is the place after it
-    v.next();
-    uint32_t segs = 0, par[2] = {0, 0};  // parity of either buffer's next P; constant indices only
-    bool ok = true;
-    auto there = [&](uint64_t* bar, uint32_t parity) { return spin(bar, parity, abort_flag); };
-    // S of 64 positions, the first or last of a tile, into the buffer of that parity
-    auto product_s = [&](int half, uint32_t kd, int b) {
-      const uint32_t qd = sw128_desc(q_s + half * L::SLOT, 16);
+      Ring<NS> v;  // V of the tile in use; K of the next one is the place after it
+      v.next();
+      uint32_t segs = 0, par[2] = {0, 0};  // parity of either buffer's next P; constant indices only
+      bool ok = true;
+      auto there = [&](uint64_t* bar, uint32_t parity) { return spin(bar, parity, abort_flag); };
+      // S of 64 positions, the first or last of a tile, into the buffer of that parity
+      auto product_s = [&](int half, uint32_t kd, int b) {
+        const uint32_t qd = sw128_desc(q_s + half * L::SLOT, 16);
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t off = ((k / 4) * L::HALF + (k % 4) * 32) >> 4;
-        mma_ss(tmem + 128 * half + STEP * b, qd + off, kd + off + ((b * STEP * 128) >> 4), IDESC_S, k > 0);
-      }
-      tc_commit(&s_full[2 * half + b]);
-    };
-    for (int at = begin; ok && at < end; ++segs) {
-      const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
-      at += g.n;
-      Ring<NS> k = v;
-      k.back();
-      ok = there(&full[k.slot], k.phase);
-#pragma unroll
-      for (int h = 0; h < MT; ++h) ok = ok && there(&q_full[h], segs & 1u);
-      if (!ok) break;
-      tc_after();
-      const uint32_t kd0 = sw128_desc(ring_s + k.slot * L::SLOT, 16);
-#pragma unroll
-      for (int h = 0; h < MT; ++h) product_s(h, kd0, 0);
-      if (g.steps > 1)
-#pragma unroll
-        for (int h = 0; h < MT; ++h) product_s(h, kd0, 1);
-      tc_commit(&empty[k.slot]);
-      for (int j = 0; ok && j < g.steps; j += 2) {
-        k.next();
-        k.next();
-        ok = there(&full[v.slot], v.phase);
-        const uint32_t kd = sw128_desc(ring_s + k.slot * L::SLOT, 16), vd0 = sw128_desc(ring_s + v.slot * L::SLOT, L::HALF);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          if (j + b >= g.steps) break;
-          const bool more = j + b + 2 < g.steps;
-#pragma unroll
-          for (int h = 0; h < MT; ++h) {
-            ok = ok && there(&p_full[2 * h + b], par[b]);
-            if (!ok) break;
-            tc_after();
-            const uint32_t p_at = tmem + 128 * h + STEP * b;
-#pragma unroll
-            for (int s = 0; s < STEP / 16; ++s) {
-              const uint32_t vs = vd0 + ((b * STEP * 128 + s * 2048) >> 4);
-              mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, b > 0 || s > 0 || j > 0);
-              if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
-            }
-            tc_commit(&o_done[2 * h + b]);
-            if (more && b == 0 && h == 0) ok = there(&full[k.slot], k.phase);
-            if (!ok) break;
-            if (more) product_s(h, kd, b);
-          }
-          par[b] ^= 1u;
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t off = ((k / 4) * L::HALF + (k % 4) * 32) >> 4;
+          mma_ss(tmem + 128 * half + STEP * b, qd + off, kd + off + ((b * STEP * 128) >> 4), IDESC_S, k > 0);
         }
-        tc_commit(&empty[v.slot]);  // both tiles' places are free once these products are done
-        if (j + 2 < g.steps) tc_commit(&empty[k.slot]);
-        v.next();
-        v.next();
+        tc_commit(&s_full[2 * half + b]);
+      };
+      for (int at = begin; ok && at < end; ++segs) {
+        const Segment g = segment_at(cut, at, end, a, shared);
+        at += g.n;
+        Ring<NS> k = v;
+        k.back();
+        ok = there(&full[k.slot], k.phase);
+#pragma unroll
+        for (int h = 0; h < MT; ++h) ok = ok && there(&q_full[h], segs & 1u);
+        if (!ok) break;
+        tc_after();
+        const uint32_t kd0 = sw128_desc(ring_s + k.slot * L::SLOT, 16);
+#pragma unroll
+        for (int h = 0; h < MT; ++h) product_s(h, kd0, 0);
+        if (g.steps > 1)
+#pragma unroll
+          for (int h = 0; h < MT; ++h) product_s(h, kd0, 1);
+        tc_commit(&empty[k.slot]);
+        for (int j = 0; ok && j < g.steps; j += 2) {
+          k.next();
+          k.next();
+          ok = there(&full[v.slot], v.phase);
+          const uint32_t kd = sw128_desc(ring_s + k.slot * L::SLOT, 16), vd0 = sw128_desc(ring_s + v.slot * L::SLOT, L::HALF);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (j + b >= g.steps) break;
+            const bool more = j + b + 2 < g.steps;
+#pragma unroll
+            for (int h = 0; h < MT; ++h) {
+              ok = ok && there(&p_full[2 * h + b], par[b]);
+              if (!ok) break;
+              tc_after();
+              const uint32_t p_at = tmem + 128 * h + STEP * b;
+#pragma unroll
+              for (int s = 0; s < STEP / 16; ++s) {
+                const uint32_t vs = vd0 + ((b * STEP * 128 + s * 2048) >> 4);
+                mma_ts(tmem + 256 + 128 * h, p_at + 8 * s, vs, IDESC_O, b > 0 || s > 0 || j > 0);
+                if constexpr (FINE) mma_ts(tmem + 256 + 128 * h, p_at + STEP / 2 + 8 * s, vs, IDESC_O, true);
+              }
+              tc_commit(&o_done[2 * h + b]);
+              if (more && b == 0 && h == 0) ok = there(&full[k.slot], k.phase);
+              if (!ok) break;
+              if (more) product_s(h, kd, b);
+            }
+            par[b] ^= 1u;
+          }
+          tc_commit(&empty[v.slot]);  // both tiles' places are free once these products are done
+          if (j + 2 < g.steps) tc_commit(&empty[k.slot]);
+          v.next();
+          v.next();
+        }
       }
-    }
-    if (!ok) {
-      *abort_flag = 1;
-      atomicOr(a.c.status, ST_TIMEOUT_FULL);
-    }
-    tc_commit(fin);  // all products are done before tensor memory is given back
-    if (!mbar_wait(fin, 0)) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(a.c.status, ST_TIMEOUT_FULL);
+      }
+      tc_commit(fin);  // all products are done before tensor memory is given back
+      if (!mbar_wait(fin, 0)) atomicOr(a.c.status, ST_TIMEOUT_DRAIN);
     }
     __syncwarp();
   } else if (warp >= 4 && warp < 4 + 4 * MT) {
@@ -336,7 +344,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     ring.next();
     bool ok = true;
     for (int at = begin; ok && at < end; ++segs) {
-      const Segment g = segment_at(cut, at, end, a.pre_rows, shared);
+      const Segment g = segment_at(cut, at, end, a, shared);
       at += g.n;
       const int base_row = g.row0 + half * 128;
       {  // a thread takes one chunk of eight elements of every (128 / CH)th row
