@@ -194,11 +194,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 
     Ring<ST> ring;
     int issued = 0;
     bool ok = true;
+    Pages pages(a.c, table, t_begin * TILE, block_hi);
     for (int t = 2 * t_begin; t < 2 * t_end; ++t) {  // K of a tile, then its V
+      const int p0 = (t >> 1) * TILE, page = pages.at(p0);
       ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
       if (!ok) break;
-      bring_tile<DP, TILE>(a.c, table, (t & 1) == 0 ? &kmap : &vmap, smem_u32(smem + ring.slot * L::SLOT), kvh, (t >> 1) * TILE, block_hi,
-                     &full[ring.slot]);
+      bring_tile<DP, TILE>(a.c, page, (t & 1) == 0 ? &kmap : &vmap, smem_u32(smem + ring.slot * L::SLOT), kvh, p0, block_hi,
+                           &full[ring.slot]);
       issued = min(issued + 1, ST);
       ring.next();
     }

@@ -9,6 +9,7 @@
 namespace ex {
 
 constexpr int TILE = 64;       // positions a tile, a multiple of 64 from position 0: a page never straddles two
+constexpr int TILE_SHIFT = 6;
 constexpr int MAX_SLOTS = 64;  // parts of a row in the shared pass, and in its own
 // Softmax weights are kept 2^P_SHIFT times as large, in o and l alike, so that f16 holds the small
 // weights of a long row in full: 2^-24 of the largest and more, where 2^-14 would be its limit.
@@ -123,6 +124,12 @@ __device__ __forceinline__ TcCut tc_cut(const AttnArgs& a, int shared) {
   return c;
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -177,24 +184,66 @@ __device__ __forceinline__ void drain(const Ring<NS>& ring, int issued, uint64_t
   if (!drained) atomicOr(status, ST_TIMEOUT_DRAIN);
 }
 
-// One warp: positions [p0, end) of head kvh, at most ROWS of them and from a multiple of ROWS, into a slot as
-// ROWS rows of 128 bytes for each 64 elements.  Boxes of rows: lane x brings the page of the x-th one.
-template <int DP, int ROWS>
-__device__ __forceinline__ void bring_tile(const KvView& c, const int32_t* table, const CUtensorMap* map, uint32_t dst, int kvh, int p0,
-                                           int end, uint64_t* bar) {
-  const int lane = threadIdx.x & 31, box = min(1 << c.ps_shift, TILE), boxes = (min(ROWS, end - p0) + box - 1) / box;
-  const int p = p0 + lane * box;
-  if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box * DP * 2);
-  __syncwarp();
-  if (lane < boxes) {
-    int page = table[p >> c.ps_shift];
-    if (page < 0 || page >= c.n_pages) {
-      atomicOr(c.status, ST_BAD_CACHE);
-      page = 0;
+// Page indices of a sequence's boxes (the rows of a page that one copy brings, 64 at most) ahead of their
+// use by a warp: lane x has that of box `first` + x, and of 32 more, so that no look-up stands between the wait
+// for a slot and the copies into it.
+struct Pages {
+  const int32_t* table;
+  int ps_shift, box_shift, end, first, now, ahead;
+  __device__ __forceinline__ Pages(const KvView& c, const int32_t* table, int p0, int end)
+      : table(table), ps_shift(c.ps_shift), box_shift(min(c.ps_shift, TILE_SHIFT)), end(end), first(p0 >> box_shift) {
+    now = look(first);
+    ahead = look(first + 32);
+  }
+  __device__ __forceinline__ int look(int box) const {
+    const long long p = static_cast<long long>(box + static_cast<int>(threadIdx.x & 31)) << box_shift;
+    return p < end ? table[p >> ps_shift] : 0;
+  }
+  // For lane x, the page of the x-th box from position p on; p never falls and steps by less than 32 boxes.
+  __device__ __forceinline__ int at(int p) {
+    const int box = p >> box_shift;
+    if (box >= first + 32) {
+      now = ahead;
+      first += 32;
+      ahead = look(first + 32);
     }
-    const int y = (kvh << c.ps_shift) + (p & ((1 << c.ps_shift) - 1));
+    return __shfl_sync(0xFFFFFFFFu, now, (box - first + (threadIdx.x & 31)) & 31);
+  }
+};
+
+// One warp: positions [p0, end) of head kvh, at most ROWS of them and from a multiple of ROWS, into a slot as
+// ROWS rows of 128 bytes for each 64 elements, by boxes of rows; lane x names the page of the x-th box.  A lane
+// brings its box where they are few.  Else one thread issues them all: a copy's operands are the warp's, so that 16
+// copies of eight lanes took 1450 cycles, of one 1050 (pages of 16: 190 -> 181 us, 32 questions behind 8k; pages of
+// 64, two boxes: 163 by lanes, 165 by one, 128 behind 32k).
+template <int DP, int ROWS>
+__device__ __forceinline__ void bring_tile(const KvView& c, int page, const CUtensorMap* map, uint32_t dst, int kvh, int p0, int end,
+                                           uint64_t* bar) {
+  const int lane = threadIdx.x & 31, box = min(1 << c.ps_shift, TILE), boxes = (min(ROWS, end - p0) + box - 1) / box;
+  const int slot_mask = (1 << c.ps_shift) - 1, head_row = kvh << c.ps_shift;
+  if (lane < boxes && (page < 0 || page >= c.n_pages)) {
+    atomicOr(c.status, ST_BAD_CACHE);
+    page = 0;
+  }
+  auto bring = [&](int x, int page_x) {
 #pragma unroll
-    for (int h = 0; h < DP / 64; ++h) tma_3d(dst + lane * box * 128 + h * ROWS * 128, map, 64 * h, y, page, bar);
+    for (int h = 0; h < DP / 64; ++h)
+      tma_3d(dst + x * box * 128 + h * ROWS * 128, map, 64 * h, head_row + ((p0 + x * box) & slot_mask), page_x, bar);
+  };
+  if (boxes <= 2) {
+    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box * DP * 2);
+    __syncwarp();
+    if (lane < boxes) bring(lane, page);
+  } else {
+    int pages[ROWS / 16];
+#pragma unroll
+    for (int x = 0; x < ROWS / 16; ++x) pages[x] = __shfl_sync(0xFFFFFFFFu, page, x);
+    if (elect_one()) {
+      mbar_arrive_expect_tx(bar, boxes * box * DP * 2);
+#pragma unroll
+      for (int x = 0; x < ROWS / 16; ++x)
+        if (x < boxes) bring(x, pages[x]);
+    }
   }
   __syncwarp();
 }

@@ -178,11 +178,13 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
       const Run r = run_at(at, i);
       at += whole ? 1 : r.n;
       const int32_t* table = a.c.table + static_cast<long long>(max(0, r.row)) * a.c.max_pages;
+      Pages pages(a.c, table, r.tile0 * TILE, r.len);
       for (int t = 2 * r.tile0; ok && t < 2 * (r.tile0 + r.n); ++t) {  // K of a tile, then its V
+        const int p0 = (t >> 1) * TILE, page = pages.at(p0);
         ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
         if (!ok) break;
-        bring_tile<DP, TILE>(a.c, table, (t & 1) == 0 ? &kmap : &vmap, smem_u32(smem + ring.slot * L::SLOT), r.kvh, (t >> 1) * TILE, r.len,
-                       &full[ring.slot]);
+        bring_tile<DP, TILE>(a.c, page, (t & 1) == 0 ? &kmap : &vmap, smem_u32(smem + ring.slot * L::SLOT), r.kvh, p0, r.len,
+                             &full[ring.slot]);
         issued = min(issued + 1, ST);
         ring.next();
       }

@@ -19,9 +19,11 @@
 // Bound: 256 rows of head_dim 128 in 16 bits against 128 positions are 2 x 4 x 128 x 128 x 128 operations:
 // 1.5 us of an SM at the rate of a large library product.  Measured: about 2.4 us, the chain from the
 // softmax's P through the issuing thread to the next S; the tensor pipe is busy 49 % of the time for 4085
-// rows of each of 8 heads on 8k positions (152 us), 57 % for 512 rows of each on 32k (112 us on 90 SMs).  Measured and not taken: steps of 128 (one buffer: 147 -> 160 us), a ring of 64 positions
-// (twice the waits and commits: 140 -> 175), the halves' waits joined (175), exponentials by polynomial
-// on 1/8 to 1/2 of the columns (+1 to +4 %).
+// rows of each of 8 heads on 8k positions (152 us), 57 % for 512 rows of each on 32k (112 us on 90 SMs).
+// Measured and not taken: steps of 128 (one buffer: 147 -> 160 us), a ring of 64 positions (twice the waits
+// and commits: 140 -> 175), the halves' waits joined (175), exponentials by polynomial on 1/8 to 1/2 of the
+// columns (+0 to +8 %), the halves' exponentials in turns, which keeps them out of phase (164 -> 172 us, 128
+// behind 32k), the prefix brought into L2 two to four tiles ahead (no difference).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -78,11 +80,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
       "r"(a), "r"(b), "r"(idesc), "r"(static_cast<int>(add)), "n"(DESC_HI)
       : "memory");
-}
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-  return p != 0;
 }
 
 #define EX_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
@@ -238,11 +235,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     for (int at = begin; ok && at < end;) {
       const Segment g = segment_at(cut, at, end, a, shared);
       at += g.n;
+      Pages pages(a.c, table, g.tile0 * TC_TILE, shared);
       for (int i = 0; ok && i < 2 * g.n; ++i) {
+        const int p0 = (g.tile0 + (i >> 1)) * TC_TILE, page = pages.at(p0);
         ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&empty[ring.slot], ring.phase ^ 1u, abort_flag)) != 0;
         if (!ok) break;
-        bring_tile<DP, TC_TILE>(a.c, table, (i & 1) == 0 ? &kmap : &vmap, smem_u32(smem + L::RING + ring.slot * L::SLOT), g.kvh,
-                                (g.tile0 + (i >> 1)) * TC_TILE, shared, &full[ring.slot]);
+        bring_tile<DP, TC_TILE>(a.c, page, (i & 1) == 0 ? &kmap : &vmap, smem_u32(smem + L::RING + ring.slot * L::SLOT), g.kvh, p0,
+                                shared, &full[ring.slot]);
         issued = min(issued + 1, NS);
         ring.next();
       }
