@@ -16,8 +16,8 @@
 // 16 rows), beside it the own pass (kvattn_one.cu for single tokens, else the rows kernel here), then the
 // join.  Floor: K and V of the prefix and of each sequence once, or 4 operations an element of K for each
 // row.  Measured, 32 query heads on 8 of 128 elements in bf16: 128 single tokens behind a prefix of 32k
-// with 33 to 2000 own positions 160 us (floor 101, bytes), 32 behind 4k with up to 511 32 us (8, bytes;
-// three kernels' latencies), 32 questions of 1 to 64 tokens behind 8k 187 us (84, operations).
+// with 33 to 2000 own positions 164 us (floor 101, bytes), 32 behind 4k with up to 511 32 us (8, bytes;
+// three kernels' latencies), 32 questions of 1 to 64 tokens behind 8k 182 us (84, operations).
 #include <cuda_runtime.h>
 
 #include <algorithm>
