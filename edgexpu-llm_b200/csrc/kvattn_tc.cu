@@ -17,7 +17,7 @@
 // accumulation, so shared memory is Q and the ring.
 //
 // Bound: 256 rows of head_dim 128 in 16 bits against 128 positions are 2 x 4 x 128 x 128 x 128 operations:
-// 1.5 us of an SM at the rate of a large library product.  Measured: 1.9 to 2.4 us, the chain from the
+// 1.5 us of an SM at the rate of a large library product.  Measured: 2.4 to 2.6 us, the chain from the
 // softmax's P through the issuing thread to the next S; the tensor pipe is busy 54 % of the time for 4085
 // rows of each of 8 heads on 8k positions (149 us), 58 % for 512 rows of each on 32k (112 us on 90 SMs).
 // Measured and not taken: steps of 128 (one buffer: 147 -> 160 us), a ring of 64 positions (twice the waits
