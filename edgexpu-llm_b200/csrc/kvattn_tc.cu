@@ -391,9 +391,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tc_wait_ld();
         const int valid = shared - g.tile0 * TC_TILE - j * STEP;
         if (valid < STEP) {
+          // -inf times a scale of 0 is no number: scores of 0 then, as all are, whose weights of 2^P_SHIFT leave the
+          // sum here (exactly) and meet values of 0 below
+          const uint32_t off = sc == 0.0f ? 0u : 0xFF800000u;
+          if (sc == 0.0f) l -= static_cast<float>((STEP - valid) << static_cast<int>(P_SHIFT));
 #pragma unroll
           for (int c = 0; c < STEP; ++c)
-            if (c >= valid) s[c] = 0xFF800000u;
+            if (c >= valid) s[c] = off;
           if (half == 0) {
             // V past the prefix's end is what memory held: 0 for the product
             ok = __all_sync(0xFFFFFFFFu, wait_or_abort(&full[ring.slot], ring.phase, abort_flag)) != 0;

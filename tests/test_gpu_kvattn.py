@@ -342,3 +342,21 @@ def test_refusals(gpu, kv):
     with pytest.raises(gpu.EdgexpuError):
         cache.attention(0, q, seqs, out_dtype=torch.bfloat16)
     assert sync_error(gpu) == ""
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 30.0])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,dim,ps,batch", [(8, 2, 64, 16, 10), (32, 8, 128, 64, 40), (12, 2, 96, 16, 50), (4, 4, 256, 32, 30)])
+@pytest.mark.parametrize("shared", [100, 130, 192])
+def test_scales_of_many_rows(kv, shared, heads, n_kv, dim, ps, batch, dtype, scale):
+    """As test_scales, with 30 to 300 rows of a key head against a prefix that ends in a tile's first half, in its
+    second, or with it: blocks of 128 and of 256 rows, and the wide heads' kernel."""
+    cache = make(kv, [shared + 1 + i % 70 for i in range(batch)], shared, heads, n_kv, dim, ps, DTYPES[dtype])
+    q = (torch.randn(batch, heads, dim, device="cuda") * 0.2).to(DTYPES[dtype])
+    seqs = list(range(1, batch + 1))
+    got = cache.attention(0, q, ints(*seqs), shared_len=shared, scale=scale)
+    want, size = reference(cache, 0, q, seqs, list(range(batch + 1)), scale)
+    # dim products of 0.2 normals and normals: sizes add up to 48 at most, a score is off by 2^-17 of that, a weight
+    # (and the sum that divides it) by as much
+    bound = (2 * UNIT[q.dtype] + 2.0 ** -15 + 2.0 ** -16 * abs(scale) * 48) * size + 2.0 ** -24
+    assert bool(((got.double() - want).abs() <= bound).all())
