@@ -114,6 +114,7 @@ _CUDA_SIGS = {
     "edgexpu_cuda_llama_forward": (_c_int, [_c_vp, _c_vp, _c_int, _c_int, ctypes.c_float, ctypes.c_float, _c_u64p,
                                             ctypes.POINTER(_c_u32), _c_vp, _c_str, _c_sz]),
     "edgexpu_cuda_llama_close": (_c_int, [_c_vp]),
+    "edgexpu_cuda_device": (_c_int, []),
     "edgexpu_cuda_kv_work_bytes": (_c_sz, [_c_int, _c_int]),
     "edgexpu_cuda_kv_append_dev": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp]),
     "edgexpu_cuda_kv_fork_dev": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_vp]),

@@ -628,6 +628,11 @@ int edgexpu_cuda_init(int device, char* error, size_t error_size) {
   return 1;
 }
 
+int edgexpu_cuda_device(void) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  return g.device;
+}
+
 int edgexpu_cuda_shutdown(void) {
   std::lock_guard<std::recursive_mutex> lk(g_mu);
   if (!g.ready) return 1;

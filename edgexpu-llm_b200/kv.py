@@ -35,6 +35,12 @@ def _load():
 _calls = _load()
 
 
+class _Desc(KvCacheDesc):
+    """The descriptor and the device of its pools, as the module reads them."""
+
+    _fields_ = [("device", ctypes.c_int)]
+
+
 class KvCache:
     """Pools k, v ``[layers][pages][kv heads][page size][head dim]`` (f16 or bf16; a page contiguous,
     layers and pages any distance apart, the same in both) and the tables over them: table int32
@@ -54,12 +60,15 @@ class KvCache:
         for t, shape, what in ((table, (n_seqs, columns), "table"), (lens, (n_seqs,), "lens"), (refs, (pages,), "refs")):
             if t.dtype != torch.int32 or t.device != k.device or t.shape != shape or not t.is_contiguous():
                 raise ValueError(f"{what}: expected contiguous int32 of shape {shape} on {k.device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+        bound = load_cuda().edgexpu_cuda_device()  # -1 before init; every call compares them again
+        if bound not in (-1, k.device.index):
+            raise ValueError(f"the cache is on {k.device}, the library on cuda:{bound}")
         size = load_cuda().edgexpu_cuda_kv_work_bytes(pages, n_seqs)
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.work = torch.empty(size // 4, dtype=torch.int32, device=k.device)
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), layer_stride, page_stride, TYPES[k.dtype], layers, pages,
-                                page, n_kv, dim, n_seqs, columns, table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
-                                self.work.data_ptr())
+        self.desc = _Desc(k.data_ptr(), v.data_ptr(), layer_stride, page_stride, TYPES[k.dtype], layers, pages,
+                          page, n_kv, dim, n_seqs, columns, table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+                          self.work.data_ptr(), k.device.index)
         self._desc = ctypes.addressof(self.desc)
 
     @classmethod
@@ -92,7 +101,7 @@ class KvCache:
 
     def compact(self):
         """Move the pages in use to the low end of the pool; how many they are, int32 on the device."""
-        return _calls.compact(self._desc, self.table)
+        return _calls.compact(self._desc)
 
     # ---- a layer of new tokens -----------------------------------------------------------------------
 

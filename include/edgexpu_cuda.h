@@ -82,6 +82,8 @@ int edgexpu_cuda_float_order(void);
 int edgexpu_cuda_init(int device, char *error, size_t error_size);
 /* Free every uploaded weight and all scratch; the library can be initialised again. */
 int edgexpu_cuda_shutdown(void);
+/* The device that the library is bound to; -1 when it is not. */
+int edgexpu_cuda_device(void);
 /* Last failure message of this process ("" if none). */
 const char *edgexpu_cuda_last_error(void);
 

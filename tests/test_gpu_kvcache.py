@@ -419,3 +419,12 @@ def test_heads_of_a_pool_past_32_bit_offsets(kv):
     assert torch.equal(k[0, 1, 0], want)
     assert cache.compact().item() == 1 and cache.table.tolist() == [[0], [-1]] and cache.refs.tolist() == [1, 0, 0]
     assert torch.equal(k[0, 0, 0], want) and torch.equal(v[0, 0, 0], (2 * x).half())
+
+
+def test_a_cache_on_another_device_than_the_librarys_is_refused(gpu, kv):
+    assert gpu.load_cuda().edgexpu_cuda_device() == 0
+    cache = filled(kv, 1, 4, 16, 1, 8, 2, 2)
+    cache.desc.device = 1  # as one that was made before the library was bound
+    for call in (lambda: cache.free(ints(0)), lambda: cache.append(ints(0), ints(1)), lambda: cache.compact()):
+        with pytest.raises(ValueError, match="the cache is on cuda:1, the library on cuda:0"):
+            call()

@@ -57,3 +57,75 @@ def test_calls_without_a_device_fail(cuda):
     assert cuda.edgexpu_cuda_kv_free_dev(ctypes.byref(desc), None, None, 0, None) == 0
     assert cuda.edgexpu_cuda_last_error()
     assert cuda.edgexpu_cuda_kv_attention_dev(ctypes.byref(desc), 0, None, None, None, 1, 1, 1, 0, 0, 1, 1.0, None, 1, None, 0, None) == 0
+
+
+@pytest.fixture(scope="module")
+def kv():
+    pkg = load_pkg()
+    pytest.importorskip("torch")
+    if not (pkg.LIB_DIR / "_kv_torch.so").exists():
+        pytest.skip("torch module not built")
+    from edgexpu_llm_b200 import kv as module
+
+    return module
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+def test_tensors_of_another_device_are_refused(kv):
+    """Each argument in turn on another GPU than the cache's, or on the host: a ValueError before any launch.  The
+    tensors are stand-ins that have a device and no memory, so none is needed here."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    if torch.cuda.device_count() == 1:
+        pytest.skip("a stand-in for a second GPU needs two where there is one")
+    with FakeTensorMode():
+        cache = kv.KvCache.empty(1, 4, 16, 1, 8, 3, 2, device="cuda:0")
+
+        def ints(n):
+            return torch.zeros(n, dtype=torch.int32, device="cuda:0")
+
+        def rows(n):
+            return torch.zeros(n, 8, device="cuda:0")
+
+        half = torch.zeros(2, 1, 8, dtype=torch.float16, device="cuda:0")
+        calls = [(cache.append, [ints(2), ints(2), ints(1)], {}), (cache.fork, [ints(2), ints(2)], {}),
+                 (cache.free, [ints(2), ints(2)], {}), (cache.copy, [ints(2), ints(2)], {}),
+                 (cache.qk_norm_rope, [0, rows(2), rows(2), rows(2), ints(2), ints(2), 1],
+                  dict(q_norm=rows(1)[0], k_norm=rows(1)[0], rope=rows(9), out=half)),
+                 (cache.attention, [0, half, ints(2)], dict(q_start=ints(3), out=half))]
+        for device in ("cuda:1", "cpu"):
+            for call, args, named in calls:
+                for at, x in list(enumerate(args)) + list(named.items()):
+                    if not isinstance(x, torch.Tensor):
+                        continue
+                    a, k = list(args), dict(named)
+                    (k if isinstance(at, str) else a)[at] = x.to(device)
+                    with pytest.raises(ValueError, match=r"on cuda:0; got .* on " + device):
+                        call(*a, **k)
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+def test_a_cache_is_made_on_the_librarys_device_alone(kv, monkeypatch):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    class Library:
+        def __init__(self, device):
+            self.edgexpu_cuda_device = lambda: device
+            self.edgexpu_cuda_kv_work_bytes = lambda pages, seqs: 64
+
+    with FakeTensorMode():
+        for bound in (-1, 0):
+            monkeypatch.setattr(kv, "load_cuda", lambda: Library(bound))
+            kv.KvCache.empty(1, 4, 16, 1, 8, 2, 2, device="cuda:0")
+        monkeypatch.setattr(kv, "load_cuda", lambda: Library(1))
+        with pytest.raises(ValueError, match="the cache is on cuda:0, the library on cuda:1"):
+            kv.KvCache.empty(1, 4, 16, 1, 8, 2, 2, device="cuda:0")
+
+
+def test_device_of_an_unbound_library(cuda):
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("another test may have bound it")
+    assert cuda.edgexpu_cuda_device() == -1
