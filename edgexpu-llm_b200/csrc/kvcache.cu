@@ -94,28 +94,29 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(const KvView c, const int3
 
 // ---- block-wide scans ---------------------------------------------------------------------------------
 
-// Exclusive sum of v over the block's threads in order; *total = the whole.  red: 33 ints.
-__device__ __forceinline__ int block_scan(int v, int* red, int* total) {
+// Exclusive sum of v over the block's threads in order; *total = the whole.  red: 33 numbers.
+template <typename I>
+__device__ __forceinline__ I block_scan(I v, I* red, I* total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  int x = v;
+  I x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    const I y = __shfl_up_sync(0xFFFFFFFFu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) red[w] = x;
   __syncthreads();
   if (w == 0) {
-    int t = lane < nw ? red[lane] : 0;
+    I t = lane < nw ? red[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xFFFFFFFFu, t, o);
+      const I y = __shfl_up_sync(0xFFFFFFFFu, t, o);
       if (lane >= o) t += y;
     }
     red[lane] = t;
   }
   __syncthreads();
-  const int r = x - v + (w > 0 ? red[w - 1] : 0);
+  const I r = x - v + (w > 0 ? red[w - 1] : 0);
   *total = red[nw - 1];
   __syncthreads();
   return r;
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
   __shared__ int s_seq[FEW ? MOST : 1], s_tail[FEW ? MOST : 1];
   __shared__ int s_list[FEW ? LIST_SHARED : 1];
   __shared__ int red[33];
+  __shared__ long long red_need[33];
   __shared__ int n_jobs;
   const Work w = work_of(c);
   const int in_page = (1 << c.ps_shift) - 1;
@@ -244,7 +246,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
   }
   __syncthreads();
   // a shared last page is copied, but for the last of the rows of the batch that share it when they are all its holders
-  int need = 0, want[PER];
+  long long need = 0;  // rows of 2^27 pages: a batch's sum passes 32 bits
+  int want[PER];
   bool split[PER];
   if constexpr (!FEW) {
 #pragma unroll
@@ -284,17 +287,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
       need += want[e];
     }
   }
-  int total;
-  int off = block_scan(need, red, &total);
+  long long total;
+  int off = static_cast<int>(block_scan(need, red_need, &total));  // read where the batch fits alone
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int b = threadIdx.x * PER + e;
     if (b < n) s_off[b] = off;
     off += want[e];
   }
-  if (threadIdx.x == 0) s_off[n] = total;
+  if (threadIdx.x == 0) s_off[n] = static_cast<int>(total);
   int32_t* list = FEW && total <= LIST_SHARED ? s_list : w.list;
-  const int found = total > 0 ? find_pages(c.refs, 0, c.n_pages, false, total, list, red) : 0;
+  const int most = static_cast<int>(min(total, static_cast<long long>(c.n_pages)));  // places of the list
+  const int found = total > 0 ? find_pages(c.refs, 0, c.n_pages, false, most, list, red) : 0;
   const bool fits = found >= total;
   __syncthreads();
   if (fits && total > 0) {  // a warp an entry: its pages into its row
@@ -330,7 +334,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_append_plan_kernel(const KvVi
   if (threadIdx.x == 0) {
     w.head[0] = n_jobs;
     if (missing != nullptr)
-      *missing = fits ? 0 : total - found;
+      *missing = fits ? 0 : static_cast<int>(min(total - found, static_cast<long long>(INT_MAX)));
     else if (!fits)
       atomicOr(c.status, ST_NO_PAGES);
   }

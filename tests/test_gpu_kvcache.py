@@ -428,3 +428,17 @@ def test_a_cache_on_another_device_than_the_librarys_is_refused(gpu, kv):
     for call in (lambda: cache.free(ints(0)), lambda: cache.append(ints(0), ints(1)), lambda: cache.compact()):
         with pytest.raises(ValueError, match="the cache is on cuda:1, the library on cuda:0"):
             call()
+
+
+@pytest.mark.parametrize("n,columns", [(3, 2 ** 27 - 1), (17, 2 ** 27 - 1), (256, 2 ** 23), (512, 2 ** 23), (300, 2 ** 23)])
+def test_a_batch_that_asks_for_more_pages_than_32_bits_count(gpu, kv, n, columns):
+    """Long rows asked for whole: their sum is 2^31 pages and more, 2^31 and 2^32 among them.  Nothing changes, and
+    the pages short are told up to 2^31 - 1."""
+    cache = filled(kv, 1, 5, 16, 1, 8, n, columns)
+    seqs, whole, missing = torch.arange(n, dtype=torch.int32, device="cuda"), ints(*[16 * columns] * n), ints(-7)
+    assert cache.append(seqs, whole, missing=missing).tolist() == [-1] * n
+    assert missing.item() == min(n * columns - 5, 2 ** 31 - 1)
+    assert not cache.lens.any() and not cache.refs.any() and int(cache.table.max()) == -1
+    assert cache.append(ints(0, 1, 2), ints(16, 32, 16), missing=missing).tolist() == [0, 0, 0] and missing.item() == 0
+    assert cache.table[:3, :2].tolist() == [[0, -1], [1, 2], [3, -1]]
+    assert sync_error(gpu) == ""
