@@ -442,3 +442,64 @@ def test_a_batch_that_asks_for_more_pages_than_32_bits_count(gpu, kv, n, columns
     assert cache.append(ints(0, 1, 2), ints(16, 32, 16), missing=missing).tolist() == [0, 0, 0] and missing.item() == 0
     assert cache.table[:3, :2].tolist() == [[0, -1], [1, 2], [3, -1]]
     assert sync_error(gpu) == ""
+
+
+def total_of(cache, model, seqs, new):
+    """Pages that an append would take."""
+    trial = Model(cache)
+    trial.rows, trial.lens, trial.refs = [list(r) for r in model.rows], list(model.lens), list(model.refs)
+    before = sum(r == 0 for r in trial.refs)
+    trial.append(seqs, new)
+    return before - sum(r == 0 for r in trial.refs)
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 1000, 4096])
+@pytest.mark.parametrize("source", [False, True])
+def test_append_of_many_forks(gpu, kv, n, source):
+    """Rows that share a partly filled last page grow by 0 to 20 tokens, n in a batch: with the row they come from the
+    batch holds all of the page's rows, without it not; with idle entries and one that comes twice; and with a page
+    too few, where nothing may change."""
+    rows = n if source else n + 1
+    rng = np.random.default_rng(n + source)
+    new = [int(x) for x in rng.choice([0, 1, 5, 20], rows)]
+    if source and n < 1000:  # all holders grow, so that one keeps the page
+        new = [max(1, x) for x in new]
+    seqs = rng.permutation(rows).tolist()
+    if not source:
+        seqs.remove(0)
+    grow = [new[s] for s in seqs]
+    probe = filled(kv, 1, 3 * rows + 4, 16, 1, 8, rows, 4)
+    model = Model(probe)
+    model.append([0], [21])
+    model.fork([0] * (rows - 1), list(range(1, rows)))
+    need = total_of(probe, model, seqs, grow) + 2
+    for short in (1, 0):
+        cache = filled(kv, 1, need - short, 16, 1, 8, rows, 4)
+        model = Model(cache)
+        cache.append(ints(0), ints(21))
+        model.append([0], [21])
+        cache.fork(ints(*[0] * (rows - 1)), ints(*range(1, rows)))
+        model.fork([0] * (rows - 1), list(range(1, rows)))
+        model.check(cache)
+        missing = ints(9)
+        got = cache.append(ints(*seqs), ints(*grow), missing=missing).tolist()
+        pos, lack = model.append(seqs, grow)
+        assert (got, missing.item()) == (pos, lack) and lack == short
+        model.check(cache)
+    assert sync_error(gpu) == ""
+    if n < 4096:  # an idle entry and one that comes twice, of which the first counts
+        cache = filled(kv, 1, need + 3 * rows, 16, 1, 8, rows, 4)
+        model = Model(cache)
+        cache.append(ints(0), ints(21))
+        model.append([0], [21])
+        cache.fork(ints(*[0] * (rows - 1)), ints(*range(1, rows)))
+        model.fork([0] * (rows - 1), list(range(1, rows)))
+        twice = seqs[n // 2]
+        got = cache.append(ints(-1, *seqs, twice), ints(7, *grow, 3)).tolist()
+        assert got == [-1] + model.append(seqs, grow)[0] + [-1]
+        model.check(cache)
+        assert "outside its cache" in sync_error(gpu)
+        got = cache.append(ints(*seqs), ints(*[1] * n)).tolist()  # rows that are apart by now, and those that are not
+        assert got == model.append(seqs, [1] * n)[0]
+        model.check(cache)
+        assert sync_error(gpu) == ""
