@@ -97,11 +97,11 @@ __device__ __noinline__ void row_again(const AttnArgs& a, const Entry& e, int kv
 // own positions.  Warp 4 brings K and V by TMA (128-byte swizzle; dims past head_dim read as 0).  Of the
 // other four, with WM = 4 each has 16 rows and all positions of a tile, with WM = 1 all have the same 16
 // rows and 16 positions of each tile, and join at the end.  P is rounded to the cache's type for its
-// product, as the tensor cores take it (with WM = 1, where bytes bound, in two numbers of the type); its
-// sum l is of the unrounded values.  Fragments of warp products, since an own pass has few rows on few
+// product, as the tensor cores take it, or (FINE: with WM = 1, where bytes bound, and where the result is fp32)
+// goes in two numbers of the type; its sum l is of the unrounded values.  Fragments of warp products, since an own pass has few rows on few
 // positions.  The own passes of 32 questions of 1 to 64 tokens on 64 to 200 positions: 41 us, bound by
 // latency, a tile's two products and its softmax in turn in each warp.
-template <typename T, int DP, int WM>
+template <typename T, int DP, int WM, bool FINE>
 __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 3)
     attn_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const int pre) {
   using L = RowsLayout<DP, WM>;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float p0v = s[i + (x >> 1)][2 * (x & 1)], p1v = s[i + (x >> 1)][2 * (x & 1) + 1];
-        if constexpr (WM == 1)
+        if constexpr (FINE)
           split16<T>(p0v, p1v, pa[x], rest[x]);
         else
           pa[x] = pack16<T>(p0v, p1v);
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, DP == 256 ? 1 : DP == 128 ? 2 : 
         vf[3] &= keep[1];
         mma16816<T>(o[2 * d], pa, vf[0], vf[1]);
         mma16816<T>(o[2 * d + 1], pa, vf[2], vf[3]);
-        if constexpr (WM == 1) {
+        if constexpr (FINE) {
           mma16816<T>(o[2 * d], rest, vf[0], vf[1]);
           mma16816<T>(o[2 * d + 1], rest, vf[2], vf[3]);
         }
@@ -667,26 +667,29 @@ size_t work_bytes(const AttnPlan& p, int n_batch, int n_tokens, int n_heads, int
   return up256(rows * 8) + up256(rows * hd * 4) + up256((static_cast<size_t>(n_batch) + 1) * 4);
 }
 
-template <typename T, int DP, int WM>
+template <typename T, int DP, int WM, bool FINE>
 cudaError_t launch_rows_as(const AttnArgs& a, uint32_t type, int blocks, int splits, int pre, cudaStream_t st) {
   using L = RowsLayout<DP, WM>;
-  static const cudaError_t set = allow_smem(attn_rows_kernel<T, DP, WM>, L::ALLOC);
+  static const cudaError_t set = allow_smem(attn_rows_kernel<T, DP, WM, FINE>, L::ALLOC);
   if (set != cudaSuccess) return set;
   CUtensorMap kmap, vmap;
   if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type))
     return cudaErrorInvalidValue;
-  return launch_dependent(attn_rows_kernel<T, DP, WM>, dim3(blocks, a.c.n_kv, splits), dim3(ROWS_THREADS), L::ALLOC, st, a, kmap, vmap, pre);
+  return launch_dependent(attn_rows_kernel<T, DP, WM, FINE>, dim3(blocks, a.c.n_kv, splits), dim3(ROWS_THREADS), L::ALLOC, st, a, kmap, vmap, pre);
+}
+
+template <typename T, int DP>
+cudaError_t launch_rows_of(const AttnArgs& a, uint32_t type, int wm, int blocks, int splits, int pre, cudaStream_t st) {
+  if (wm == 1) return launch_rows_as<T, DP, 1, true>(a, type, blocks, splits, pre, st);
+  return a.out_f32 ? launch_rows_as<T, DP, 4, true>(a, type, blocks, splits, pre, st)
+                   : launch_rows_as<T, DP, 4, false>(a, type, blocks, splits, pre, st);
 }
 
 template <typename T>
 cudaError_t launch_rows(const AttnArgs& a, uint32_t type, int wm, int blocks, int splits, int pre, cudaStream_t st) {
-  if (wm == 1)
-    return a.c.hd <= 64    ? launch_rows_as<T, 64, 1>(a, type, blocks, splits, pre, st)
-           : a.c.hd <= 128 ? launch_rows_as<T, 128, 1>(a, type, blocks, splits, pre, st)
-                           : launch_rows_as<T, 256, 1>(a, type, blocks, splits, pre, st);
-  return a.c.hd <= 64    ? launch_rows_as<T, 64, 4>(a, type, blocks, splits, pre, st)
-         : a.c.hd <= 128 ? launch_rows_as<T, 128, 4>(a, type, blocks, splits, pre, st)
-                         : launch_rows_as<T, 256, 4>(a, type, blocks, splits, pre, st);
+  return a.c.hd <= 64    ? launch_rows_of<T, 64>(a, type, wm, blocks, splits, pre, st)
+         : a.c.hd <= 128 ? launch_rows_of<T, 128>(a, type, wm, blocks, splits, pre, st)
+                         : launch_rows_of<T, 256>(a, type, wm, blocks, splits, pre, st);
 }
 
 template <typename T>

@@ -8,8 +8,10 @@
 // S a half of the rows, and two halves with MT = 2: products of one run while another is in its softmax,
 // and both halves read the same tiles of K and V.  A row's reference maximum moves only when the maximum
 // has grown by more than GROW (in log2 units); then O and the sum are rescaled, which after the first
-// tiles is rare.  P is rounded to the cache's type for its product (with MT = 1, where bytes bound, in
-// two numbers of the type); its sum l, S and O are fp32.
+// tiles is rare.  P goes to its product in two numbers of the cache's type where bytes bound (MT = 1) or the
+// result is fp32, which a weight rounded to the type would not bear; else rounded to the type, 2^-8 (bf16) or
+// 2^-11 (f16) of a weight at most, since the second product costs 185 -> 204 us (128 tokens behind 32k) and 188 -> 255
+// (32 questions behind 8k).  Its sum l, S and O are fp32.
 //
 // Warps: 0 brings K and V by TMA (a box a page and 64 elements; 128-byte swizzle) through a ring of
 // slots of 128 positions, one thread of 1 issues the products, 4..7 and 8..11 are the rows.  S, P:
@@ -169,12 +171,12 @@ __device__ __forceinline__ Segment segment_at(const TcCut& c, int at, int end, c
   return s;
 }
 
-template <typename T, int DP, int MT>
+// FINE: P in two numbers of the type, a coarse and the rest.
+template <typename T, int DP, int MT, bool FINE>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using L = TcLayout<DP, MT>;
   constexpr int CH = DP / 8, NS = L::SLOTS;
-  constexpr bool FINE = MT == 1;  // P in two numbers of the type, a coarse and the rest
   constexpr uint32_t FMT = exponent16<T>() == exponent16<__half>() ? 0u : 1u;
   // D fp32, A and B of the type, M = 128; N = 64 for S, DP for O, whose B is read across its rows
   constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t(STEP) >> 3) << 17) | ((128u >> 4) << 24);
@@ -553,20 +555,25 @@ bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t 
 
 namespace {
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, bool FINE>
 cudaError_t launch_tc_as(const AttnArgs& a, uint32_t type, cudaStream_t st) {
   using L = TcLayout<DP, MT>;
-  static const cudaError_t set = allow_smem(attn_tc_kernel<T, DP, MT>, L::ALLOC);
+  static const cudaError_t set = allow_smem(attn_tc_kernel<T, DP, MT, FINE>, L::ALLOC);
   if (set != cudaSuccess) return set;
   CUtensorMap kmap, vmap;
   if (!pool_map(&kmap, a.c.k + a.layer_off, a.c, type) || !pool_map(&vmap, a.c.v + a.layer_off, a.c, type)) return cudaErrorInvalidValue;
-  return launch_dependent(attn_tc_kernel<T, DP, MT>, dim3(a.pre_ctas), dim3(TC_THREADS), L::ALLOC, st, a, kmap, vmap);
+  return launch_dependent(attn_tc_kernel<T, DP, MT, FINE>, dim3(a.pre_ctas), dim3(TC_THREADS), L::ALLOC, st, a, kmap, vmap);
+}
+
+template <typename T, int DP>
+cudaError_t launch_tc_rows(const AttnArgs& a, uint32_t type, cudaStream_t st) {
+  if (a.pre_rows == 128) return launch_tc_as<T, DP, 1, true>(a, type, st);
+  return a.out_f32 ? launch_tc_as<T, DP, 2, true>(a, type, st) : launch_tc_as<T, DP, 2, false>(a, type, st);
 }
 
 template <typename T>
 cudaError_t launch_tc(const AttnArgs& a, uint32_t type, cudaStream_t st) {
-  if (a.c.hd <= 64) return a.pre_rows == 128 ? launch_tc_as<T, 64, 1>(a, type, st) : launch_tc_as<T, 64, 2>(a, type, st);
-  return a.pre_rows == 128 ? launch_tc_as<T, 128, 1>(a, type, st) : launch_tc_as<T, 128, 2>(a, type, st);
+  return a.c.hd <= 64 ? launch_tc_rows<T, 64>(a, type, st) : launch_tc_rows<T, 128>(a, type, st);
 }
 
 }  // namespace

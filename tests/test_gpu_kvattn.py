@@ -360,3 +360,25 @@ def test_scales_of_many_rows(kv, shared, heads, n_kv, dim, ps, batch, dtype, sca
     # (and the sum that divides it) by as much
     bound = (2 * UNIT[q.dtype] + 2.0 ** -15 + 2.0 ** -16 * abs(scale) * 48) * size + 2.0 ** -24
     assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,dim,ps,shared,n_q,own", [
+    (32, 8, 128, 64, 1000, None, 33), (32, 8, 128, 64, 700, [64, 1, 17, 40], 3), (9, 3, 64, 16, 300, [100, 50], 0),
+    (12, 2, 96, 16, 0, [70, 33], 20), (4, 4, 256, 32, 500, [30, 70], 5), (34, 2, 64, 16, 0, None, 900)])
+def test_fp32_output_keeps_the_weights_to_16_bits_and_more(kv, heads, n_kv, dim, ps, shared, n_q, own, dtype):
+    """fp32 out: the weights go to their product in two numbers of the type, whichever kernel makes it, so that they
+    are off by 2^-15 (bf16) or 2^-20 (f16), or by 2^-33 of the row's largest; sums, scores and exponentials as above."""
+    count = n_q or [1] * 70
+    lens = [shared + n + own + i % 50 for i, n in enumerate(count)]
+    cache = make(kv, lens, shared, heads, n_kv, dim, ps, DTYPES[dtype], seed=dim)
+    starts = [sum(count[:i]) for i in range(len(count) + 1)]
+    q = torch.randn(starts[-1], heads, dim, device="cuda").to(DTYPES[dtype])
+    seqs = list(range(1, len(lens) + 1))
+    got = cache.attention(0, q, ints(*seqs), q_start=ints(*starts) if n_q else None, shared_len=shared, scale=dim ** -0.5,
+                          out_dtype=torch.float32)
+    want, size = reference(cache, 0, q, seqs, starts, dim ** -0.5)
+    weights = 2.0 ** -15 if dtype == "bf16" else 2.0 ** -20
+    bound = (weights + 2.0 ** -15) * size + max(lens) * 2.0 ** -33 * 6  # values of at most 6
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
