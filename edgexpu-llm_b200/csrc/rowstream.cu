@@ -23,6 +23,7 @@ cudaError_t launch_rowstream(const RowStreamArgs& in, const DeviceInfo& dev, cud
     if (a.n_seg > MAX_SEGS || a.mode != RowOut::Store) return cudaErrorInvalidValue;
     a.n_rows = 0;
     for (int i = 0; i < a.n_seg; ++i) a.n_rows += a.seg[i].n_rows;
+    a.out_stride = a.seg[0].n_rows;  // of a group of one, which the kernel takes for a lone tensor
   }
   if (a.mode == RowOut::StoreTp && (a.tp.world < 2 || a.tp.world > TP_MAX_WORLD ||
                                     (a.fmt != Fmt::Q8_0xQ8_0 && a.fmt != Fmt::Q4_KxQ8_K)))

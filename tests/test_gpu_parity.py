@@ -406,3 +406,26 @@ def test_multi_tensor_launch_equals_separate_calls(gpu, port, wtype, m):
     finally:
         for h in hs:
             gpu.free_weight(h)
+
+
+@pytest.mark.parametrize("wtype", [TYPE_Q4_K, TYPE_Q8_0])
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 20])
+def test_multi_tensor_launch_of_one_tensor(gpu, wtype, m):
+    """A group of one: every row in its own place, as by the call for one tensor."""
+    torch = _torch()
+    s = _synth()
+    rng = np.random.default_rng(m)
+    n_out, n_in = 320, 768
+    h = gpu.upload_weight(s.weight(rng, wtype, n_out, n_in), wtype, n_out, n_in)
+    try:
+        x = torch.from_numpy(s.activations(rng, m, n_in)).cuda()
+        out, want = (torch.full((m, n_out), float("nan"), device="cuda") for _ in range(2))
+        cuda = gpu.load_cuda()
+        P = ctypes.c_void_p * 1
+        assert cuda.edgexpu_cuda_linear_quant_multi_dev(1, P(out.data_ptr()), P(h), (ctypes.c_int * 1)(n_out), None, wtype, x.data_ptr(),
+                                                        m, n_in, _stream()), cuda.edgexpu_cuda_last_error()
+        assert cuda.edgexpu_cuda_linear_quant_batch_dev(want.data_ptr(), x.data_ptr(), h, wtype, None, m, n_out, n_in, _stream())
+        _sync(gpu)
+        np.testing.assert_array_equal(out.cpu().numpy(), want.cpu().numpy())
+    finally:
+        gpu.free_weight(h)
