@@ -594,7 +594,7 @@ struct AttnPlan {
 
 AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n_heads, int shared_len, int max_len) {
   AttnPlan p{};
-  const int sms = api_device_info().sm_count > 0 ? api_device_info().sm_count : 148;
+  const int sms = attn_sms();
   const int rep = n_heads / n_kv;
   const long long rows = static_cast<long long>(n_tokens) * rep;
   shared_len = std::max(0, std::min(shared_len, max_len));
@@ -705,7 +705,7 @@ cudaError_t launch_attention_as(const AttnArgs& a, const AttnPlan& p, uint32_t t
   if (e != cudaSuccess || part_rows(p, a.n_tokens, a.n_heads) == 0) return e;
   // a head a warp while that leaves warps free, else several: what a token needs is looked up once for them
   const long long rows = static_cast<long long>(a.n_tokens) * a.n_heads;
-  const int heads = rows <= 32LL * api_device_info().sm_count ? 1 : 4, per_token = (a.n_heads + heads - 1) / heads;
+  const int heads = rows <= 32LL * attn_sms() ? 1 : 4, per_token = (a.n_heads + heads - 1) / heads;
   const unsigned blocks = static_cast<unsigned>((static_cast<long long>(a.n_tokens) * per_token + 3) / 4);
   return launch_dependent(a.c.hd > 128 ? attn_join_kernel<T, true, 4> : heads == 1 ? attn_join_kernel<T, false, 8> : attn_join_kernel<T, false, 4>, dim3(blocks), dim3(128), 0, st, a,
                           heads, per_token);

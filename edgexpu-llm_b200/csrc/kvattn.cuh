@@ -4,6 +4,7 @@
 
 #include <cuda.h>
 
+#include "capi_internal.h"
 #include "kv.cuh"
 
 namespace ex {
@@ -147,6 +148,13 @@ __device__ __forceinline__ float ex2(float x) {
 // A layer of a pool as [page][head x slot][element], in boxes of 64 elements of at most 64 of a page's
 // positions; elements past head_dim read as 0 (kvattn_tc.cu).
 bool pool_map(CUtensorMap* map, const uint16_t* base, const KvView& c, uint32_t type);
+
+// SMs for the division of the work: the device's, or a B200's before the library is bound to one, so that a work
+// size asked for then holds.
+inline int attn_sms() {
+  const int n = api_device_info().sm_count;
+  return n > 0 ? n : 148;
+}
 
 // Launch the single tokens' own pass (kvattn_one.cu), hd at most 128; its blocks where the line is cut.
 constexpr int ONE_MAX_BATCH = 1024;  // what the runs need is in shared memory

@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
 template <int DP>
 int blocks_of(int rep, int n_batch, long long tiles, int free_sms) {
   const size_t smem = one_smem<DP>(std::min(16, rep), n_batch, false);
-  const int fit = std::max(1, std::min(static_cast<int>((228 * 1024) / (smem + 1024)), 2)), all = fit * api_device_info().sm_count;
+  const int fit = std::max(1, std::min(static_cast<int>((228 * 1024) / (smem + 1024)), 2)), all = fit * attn_sms();
   return 2 * (tiles >= 32LL * all ? all : fit * free_sms);
 }
 

@@ -7,6 +7,9 @@ weight for the standard normal heads here), and u |out| + 2^-24 for the output's
 """
 
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import pytest
 
@@ -382,3 +385,21 @@ def test_fp32_output_keeps_the_weights_to_16_bits_and_more(kv, heads, n_kv, dim,
     bound = (weights + 2.0 ** -15) * size + max(lens) * 2.0 ** -33 * 6  # values of at most 6
     err = (got.double() - want).abs()
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+def test_work_bytes_are_the_same_before_and_after_init():
+    code = """
+import ctypes, itertools, sys
+sys.path.insert(0, {tests!r})
+from _oracle import load_pkg
+pkg = load_pkg()
+f = pkg.load_cuda().edgexpu_cuda_kv_attention_work_bytes
+def sizes():
+    return [f(ctypes.byref(pkg.KvCacheDesc(n_kv=n_kv, head_dim=dim)), batch, batch * each, 4 * n_kv, shared, shared + more)
+            for n_kv, dim, batch, each, shared, more in itertools.product((1, 8), (64, 128, 256), (1, 30, 128, 1100), (1, 7), (0, 100, 32768), (1, 700, 20000))]
+before = sizes()
+pkg.init(0)
+assert sizes() == before
+pkg.shutdown()
+"""
+    subprocess.run([sys.executable, "-c", code.format(tests=str(pathlib.Path(__file__).parent))], check=True, timeout=300)

@@ -47,6 +47,15 @@ def test_attention_work_bytes(cuda):
     assert cuda.edgexpu_cuda_kv_attention_work_bytes(None, 1, 1, 1, 0, 1) == 0
 
 
+def test_attention_work_bytes_before_the_library_is_bound(cuda):
+    """128 single tokens on up to 32000 positions of their own: the line of tiles is cut for a B200's SMs, 16 rows
+    that continue an earlier block's run for each block, at least one block an SM."""
+    pkg = load_pkg()
+    desc = pkg.KvCacheDesc(n_kv=8, head_dim=128)
+    need = cuda.edgexpu_cuda_kv_attention_work_bytes(ctypes.byref(desc), 128, 128, 32, 0, 32000)
+    assert need >= (128 * 32 + 16 * 148) * (128 * 4 + 8)
+
+
 def test_calls_without_a_device_fail(cuda):
     import torch
 
