@@ -5,6 +5,7 @@ import ctypes
 import pathlib
 import re
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -97,3 +98,17 @@ def test_linear_without_device_writes_nan_and_sticky_error(built):
     assert np.all(out == 1.0) and host.edgexpu_b200_last_error() == b""
     q = np.zeros(34, np.uint8)
     assert host.edgexpu_gguf_quantize_q8_0(x.ctypes.data, 32, q.ctypes.data) == 0
+
+
+def test_the_libraries_build_without_torch():
+    """The recipe, not run: with an interpreter that has no torch the C libraries alone and a note, with one that has
+    it the torch module too."""
+    pytest.importorskip("torch")
+    make = ["make", "-n", "-B", "-C", str(load_pkg().PKG_DIR)]
+    without, none = (subprocess.run(make + [f"PYTHON={python}"], capture_output=True, text=True, check=True).stdout
+                     for python in (sys.executable + " -S -I", "/no/such/python"))
+    for out in (without, none):
+        assert "libedgexpu_cuda.so" in out and "libedgexpu_b200_host.so" in out
+        assert "kv_torch.cpp" not in out and "is left out" in out
+    both = subprocess.run(make + [f"PYTHON={sys.executable}"], capture_output=True, text=True, check=True).stdout
+    assert "kv_torch.cpp" in both and "is left out" not in both
