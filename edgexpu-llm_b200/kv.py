@@ -3,7 +3,9 @@
 :class:`KvCache` binds the ``edgexpu_cuda_kv_*`` and ``edgexpu_cuda_qk_norm_rope_dev`` calls of
 ``include/edgexpu_cuda.h``, which say what each call does.  Tensors live on the library's device and
 calls run on torch's current stream; none of them waits for the device.  A tensor of another type, shape
-or device is a ValueError, a call that the library refuses an EdgexpuError.
+or device is a ValueError, a call that the library refuses an EdgexpuError.  What only the device finds (a
+sequence or page outside its cache, too few free pages, a wait that ran out) is an EdgexpuError of the next
+:meth:`KvCache.synchronize`; torch's own synchronisation does not tell.
 """
 
 from __future__ import annotations
@@ -13,7 +15,7 @@ import importlib.util
 
 import torch
 
-from . import LIB_DIR, PKG_DIR, TYPE_BF16, TYPE_F16, EdgexpuError, KvCacheDesc, load_cuda
+from . import LIB_DIR, PKG_DIR, TYPE_BF16, TYPE_F16, EdgexpuError, KvCacheDesc, _check, _err_buf, load_cuda
 
 TYPES = {torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 PAIRINGS = {"adjacent": 0, "halves": 1}
@@ -79,6 +81,12 @@ class KvCache:
         return cls(k, v, torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=device),
                    torch.zeros(n_seqs, dtype=torch.int32, device=device),
                    torch.zeros(n_pages, dtype=torch.int32, device=device))
+
+    def synchronize(self) -> None:
+        """Wait for torch's current stream and raise what calls of the process, this cache's among them, found wrong
+        on the device since the last time."""
+        buf = _err_buf()
+        _check(load_cuda().edgexpu_cuda_stream_sync(torch.cuda.current_stream(self.k.device).cuda_stream, buf, 512), buf)
 
     # ---- pages -------------------------------------------------------------------------------------
 

@@ -160,11 +160,12 @@ def main():
         torch.cuda.synchronize()
         t = time.perf_counter()
         out = generate(model, cache, prompt, questions, new_tokens, share)
-        torch.cuda.synchronize()
+        cache.synchronize()  # and what the calls found wrong on the device
         print(f"prompt {'read once for all' if share else 'read by each'}: {time.perf_counter() - t:.3f} s, "
               f"first ids {out[0, :6].tolist()}, pages in use {int((cache.refs > 0).sum())}")
         cache.free(ints(list(range(1, requests // 2 + 1))))
         print(f"  half of the requests given back, pages in use after packing: {int(cache.compact())}")
+        cache.synchronize()
     model.close()
     pkg.shutdown()
 

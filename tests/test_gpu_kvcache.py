@@ -503,3 +503,18 @@ def test_append_of_many_forks(gpu, kv, n, source):
         assert got == model.append(seqs, [1] * n)[0]
         model.check(cache)
         assert sync_error(gpu) == ""
+
+
+def test_synchronize_raises_what_the_device_found(gpu, kv):
+    cache = filled(kv, 1, 4, 16, 1, 64, 2, 6)
+    x = torch.randn(1, 64, device="cuda")
+    cache.synchronize()
+    for call, word in [(lambda: cache.append(ints(0), ints(80)), "too few free pages"), (lambda: cache.free(ints(2)), "outside its cache"),
+                       (lambda: cache.qk_norm_rope(0, x, x, x, ints(1), ints(0), n_heads=1), "outside its cache"),
+                       (lambda: cache.attention(0, x.half().reshape(1, 1, 64), ints(7)), "outside its cache")]:
+        for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+            with torch.cuda.stream(stream):
+                call()
+                with pytest.raises(gpu.EdgexpuError, match=word):
+                    cache.synchronize()
+                cache.synchronize()  # told once
