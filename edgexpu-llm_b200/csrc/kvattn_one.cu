@@ -370,13 +370,15 @@ __global__ void __launch_bounds__(ONE_THREADS, 2)
 }
 
 // Two rounds of blocks: SMs do not get the same share of a busy memory, and the second round evens that out.
-// Of all SMs where each block gets 16 tiles and more (128 sequences of 33 to 2000 positions: one round 185
-// us, two 182), else of those that the shared pass leaves (32 behind 4k: one round 35.6 us, two 32.4).
+// Of the SMs that the shared pass leaves (32 behind 4k: one round 35.6 us, two 32.4), but no block gets more than 16
+// tiles before there are two rounds of all SMs (128 sequences of 33 to 2000 positions: one round 185 us, two 182):
+// where the shared pass leaves few, the blocks past the first round wait for its end and then have every SM (128
+// behind 32k with up to 224 of their own and two SMs left: 16 blocks 321 us, 320 blocks 114).
 template <int DP>
 int blocks_of(int rep, int n_batch, long long tiles, int free_sms) {
   const size_t smem = one_smem<DP>(std::min(16, rep), n_batch, false);
   const int fit = std::max(1, std::min(static_cast<int>((228 * 1024) / (smem + 1024)), 2)), all = fit * attn_sms();
-  return 2 * (tiles >= 32LL * all ? all : fit * free_sms);
+  return std::max(2 * fit * free_sms, static_cast<int>(std::min(2LL * all, (tiles + 15) / 16)));
 }
 
 template <typename T, int DP>

@@ -56,6 +56,27 @@ def test_attention_work_bytes_before_the_library_is_bound(cuda):
     assert need >= (128 * 32 + 16 * 148) * (128 * 4 + 8)
 
 
+def test_single_tokens_pieces_stay_short_where_the_shared_pass_leaves_few_sms(cuda):
+    """128 single tokens behind 32k, 148 SMs: the shared pass takes all of them with up to 192 own positions and all but
+    two with 224 and 256; the own pass's blocks get 16 tiles at most all the same, or there are four an SM."""
+    pkg = load_pkg()
+    desc = pkg.KvCacheDesc(n_kv=8, head_dim=128)
+    slot = 128 * 32  # rows of a part: tokens x heads
+
+    def rows(own):
+        size = cuda.edgexpu_cuda_kv_attention_work_bytes(ctypes.byref(desc), 128, 128, 32, 32768, 32768 + own)
+        up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+        return next(r for r in range(size // 520, 0, -1) if up(r * 8) + up(r * 512) + up(129 * 4) == size)
+
+    # as many parts with 224 and 256, for 72 to 74 pieces of a line of 8
+    parts = (rows(192) - 16 * 4 * 148) // slot
+    assert parts * slot + 16 * 4 * 148 == rows(192)
+    for own in (224, 256):
+        tiles = 128 * 8 * ((own + 63) // 64 + 1)
+        blocks = (rows(own) - parts * slot) // 16
+        assert blocks >= min(4 * 148, tiles // 16), (own, blocks, tiles)
+
+
 def test_calls_without_a_device_fail(cuda):
     import torch
 
