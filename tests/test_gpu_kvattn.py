@@ -403,3 +403,18 @@ assert sizes() == before
 pkg.shutdown()
 """
     subprocess.run([sys.executable, "-c", code.format(tests=str(pathlib.Path(__file__).parent))], check=True, timeout=300)
+
+
+@pytest.mark.parametrize("n_q,batch", [(None, 160), ([300], 1)])
+def test_more_blocks_of_rows_than_half_the_sms(kv, n_q, batch):
+    """130 heads on one key head: 78 blocks of 256 rows and more, which then go along the prefix one after the other."""
+    lens = [200 + (n_q[0] if n_q else 1) + i % 40 for i in range(batch)]
+    run(kv, lens, 200, 130, 1, 64, 16, "bf16", n_q=n_q)
+    run(kv, lens, 200, 130, 1, 128, 64, "f16", n_q=n_q, out_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("batch", [1023, 1024, 1025, 1100])
+def test_a_thousand_single_tokens(kv, batch):
+    """Around the number of entries up to which single tokens have a kernel of their own."""
+    for shared, more in ((0, 40), (70, 1), (70, 130)):
+        run(kv, [shared + more + i % 30 for i in range(batch)], shared, 2, 1, 64, 16, "f16", max_len=shared + more + 700)
