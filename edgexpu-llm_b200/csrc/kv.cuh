@@ -79,9 +79,10 @@ __host__ __device__ constexpr uint32_t exponent16<__nv_bfloat16>() {
   return 0x7F80u;
 }
 
-// Two weights >= 0 as a coarse number of the type each and the rest, both above 0 where the weight is (a
-// product of either with an infinity then has its sign): the coarse one is rounded from a little less
-// than the weight.  Together they hold it to 2^-16 (bf16) or 2^-20 (f16).
+// Two weights >= 0 as a coarse number of the type each and the rest, which is never below 0: the coarse one is
+// rounded from a little less than the weight.  Together they hold it to 2^-15 (bf16), or to 2^-20 or, below 2^-5,
+// 2^-25 (f16).  Down to 2^-115 (bf16) or 2^-14 (f16: with P_SHIFT 2^-24 of the row's largest) both are above 0, so
+// that their products with an infinity have its sign; a smaller weight may make NaN of it.
 template <typename T>
 __device__ __forceinline__ void split16(float p0, float p1, uint32_t& coarse, uint32_t& rest) {
   constexpr float LESS = exponent16<T>() == 0x7C00u ? 1.0f - 1.0f / 1024 : 1.0f - 1.0f / 256;

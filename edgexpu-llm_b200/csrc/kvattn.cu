@@ -15,9 +15,11 @@
 // Launches: the shared pass (kvattn_tc.cu; the rows kernel here for heads above 128 elements or at most
 // 16 rows), beside it the own pass (kvattn_one.cu for single tokens, else the rows kernel here), then the
 // join.  Floor: K and V of the prefix and of each sequence once, or 4 operations an element of K for each
-// row.  Measured, 32 query heads on 8 of 128 elements in bf16: 128 single tokens behind a prefix of 32k
-// with 33 to 2000 own positions 164 us (floor 101, bytes), 32 behind 4k with up to 511 32 us (8, bytes;
-// three kernels' latencies), 32 questions of 1 to 64 tokens behind 8k 182 us (84, operations).
+// row.  Measured, 32 query heads on 8 of 128 elements, calls back to back with inputs in rotation: 128 single tokens
+// behind a prefix of 32k with 33 to 2000 own positions in f16 189 us (floor 101, bytes), 32 behind 4k with up to 511
+// in bf16 33 us (8, bytes; three kernels' latencies), 32 questions of 1 to 64 tokens behind 8k in f16 194 us (84,
+// operations).  The same inputs for some milliseconds: 167, 32 and 182 to 191 us; the changes' figures below and in
+// the other files are of that kind.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -621,8 +623,10 @@ AttnPlan plan_of(int n_kv, int hd, bool ragged, int n_batch, int n_tokens, int n
     const long long blocks = (rows + p.pre_rows - 1) / p.pre_rows * n_kv;
     // Beside single tokens the shared pass takes its share of the SMs, by measured costs of SM time: 2.6 us a tile of 256
     // rows, 1.6 of 128, 0.5 a tile of the own passes (taken half as long as they may be), and a tenth more, since the own
-    // pass goes on where the shared one has ended.  128 behind 32k: 184 -> 169 us, 32 behind 4k: 37 -> 32.  Several
-    // tokens' own passes want all SMs after it instead (shares of 0.6 and 0.85 of them: 192 -> 256, 198 us).
+    // pass goes on where the shared one has ended.  128 behind 32k: 184 -> 169 us, 32 behind 4k: 37 -> 32.  The costs are
+    // those of heads of 128; with the same numbers for 64 and 96 elements and pages of 16, 1.1 is within 5 % of the best
+    // of 0.7 to 1.8 in eight of nine layouts, and 36.6 us against 31.3 (0.9) for 64 tokens of 12 heads on 2 of 96 behind
+    // 8k.  Several tokens' own passes want all SMs after it instead (shares of 0.6 and 0.85 of them: 192 -> 256, 198 us).
     double share = 1.0;
     if (p.one) {
       const double pre = static_cast<double>(blocks) * tiles * (p.pre_rows == 256 ? 2.6 : 1.6);

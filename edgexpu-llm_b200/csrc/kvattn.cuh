@@ -9,7 +9,7 @@
 
 namespace ex {
 
-constexpr int TILE = 64;       // positions a tile, a multiple of 64 from position 0: a page never straddles two
+constexpr int TILE = 64;       // positions a tile, a multiple of 64 from position 0: a box of a page, 64 positions at most, never straddles two
 constexpr int TILE_SHIFT = 6;
 constexpr int MAX_SLOTS = 64;  // parts of a row in the shared pass, and in its own
 // Softmax weights are kept 2^P_SHIFT times as large, in o and l alike, so that f16 holds the small

@@ -162,7 +162,9 @@ __device__ int find_pages(const int32_t* refs, int from, int to, bool live, int 
 // One block: what each entry needs, the lowest free pages for it, and the last pages to be copied.  Bound by
 // latency, a chain of dependent loads and block barriers.  FEW: at most 256 entries, one a thread; which
 // entry names a sequence first and which rows of the batch share a last page is then found by comparing
-// all pairs in shared memory, else by atomics in `work` (64 entries: 8 us there, 5 here).
+// all pairs in shared memory, else by atomics in `work`.  Free and append, three kernels in a graph, of 16, 64, 128
+// and 256 entries: 6.7, 7.6, 8.6 and 10.5 us by pairs, 10.3, 11.3, 11.8 and 12.9 in `work`; with a fork between them
+// 10.0, 11.0, 12.9 and 16.0 against 13.7, 14.3, 16.0 and 16.4.
 constexpr int APPEND_FEW = 256;
 constexpr int LIST_SHARED = 2048;  // pages found, in shared memory up to so many
 
@@ -349,8 +351,8 @@ constexpr int PIECE = 4096;  // bytes a warp copies at once: eight 16-byte loads
 //   stride 1: job i is src[i] -> dst[i], all tokens; stride 3: jobs[3i], jobs[3i + 1], jobs[3i + 2] tokens.
 //   n_dev: the number of jobs, on the device; else n.
 //   remap: afterwards table entries p >= *n_dev_live become remap[p] (a packing).
-// A packing of 48 sequences of up to 4000 tokens (1.7 GB each way) 546 us, 95 % of a copy's rate; 127 copies of
-// one last page (0.5 GB written, 4 MB read) 88 us.
+// A packing of 48 sequences of up to 4000 tokens (1.7 GB each way) 546 us, 95 % of a copy's rate; 128 copies of
+// one last page (0.53 GB written, 4 MB read) 88 us.
 struct MoveArgs {
   const int32_t* src;
   const int32_t* dst;

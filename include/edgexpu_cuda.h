@@ -397,7 +397,8 @@ int edgexpu_cuda_qk_norm_rope_dev(const edgexpu_cuda_kv_cache *cache, int layer,
  * EDGEXPU_CUDA_TYPE_F32 (the next linear's input).  Products are of the cache's type, sums are fp32.  With an
  * fp32 out every softmax weight goes to its product in two numbers of that type, which hold it to 2^-15 (bf16) or
  * 2^-20 (f16; or to 2^-35 of the row's largest weight); with an out of the cache's type it may be
- * rounded to the type, as the result is.  max_len bounds the sequences' lengths for the division of the work
+ * rounded to the type, as the result is.  (An infinity in V whose weight is below 2^-24 of the row's largest may give
+ * NaN.)  max_len bounds the sequences' lengths for the division of the work
  * only.  work: edgexpu_cuda_kv_attention_work_bytes bytes of device memory, 256-byte aligned, of this call's own until it
  * is done; the size depends on these numbers alone and may be 0. */
 int edgexpu_cuda_kv_attention_dev(const edgexpu_cuda_kv_cache *cache, int layer, const void *q, const int32_t *seqs,
